@@ -48,3 +48,22 @@ def core():
                 f"in the repository root ({e})") from e
         _core = m
     return _core
+
+
+_ops = None
+
+
+def ops():
+    """The serving operators (``tilelang/_tl_ops*.so`` from csrc/ops): hand-written gfx950 kernels and
+    their host forms.  There is no other implementation behind them."""
+    global _ops
+    if _ops is None:
+        try:
+            import torch  # noqa: F401  (loads libc10_hip.so, which the extension links against)
+            from . import _tl_ops as m  # noqa: F401
+        except ImportError as e:
+            raise NativeRuntimeMissing(
+                "tilelang serving operators not built: run `python setup.py build_ext --inplace` "
+                f"in the repository root ({e})") from e
+        _ops = m
+    return _ops

@@ -6,7 +6,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 
 
 def find_lib_path(name: str = "_tl_runtime"):
-    """Paths of the in-tree extension modules matching ``name`` (``_tl_runtime`` / ``_tl_core``)."""
+    """Paths of the in-tree extension modules matching ``name`` (``_tl_runtime`` / ``_tl_core`` / ``_tl_ops``)."""
     return sorted(glob.glob(os.path.join(_HERE, f"{name}*.so")))
 
 

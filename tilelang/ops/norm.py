@@ -1,12 +1,15 @@
-"""Fused RMSNorm (reference counterpart: examples/norm/rms_norm.py and the model's ``RMSNorm``)."""
+"""Fused RMSNorm (reference counterpart: examples/norm/rms_norm.py and the model's ``RMSNorm``), and
+its form in front of the block-scaled fp8 GEMMs: residual addition, norm and e4m3 quantisation in one pass."""
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple, Optional
 
 import torch
 
 import tilelang
 import tilelang.language as T
+from tilelang import _native
 
 
 @functools.lru_cache(maxsize=None)
@@ -66,3 +69,28 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.
     dt = {torch.float16: "float16", torch.bfloat16: "bfloat16", torch.float32: "float32"}[x2.dtype]
     k = _rms_kernel(M, N, dt, float(eps), "cpu" if x2.device.type == "cpu" else "hip")
     return k(x2, weight.to(x2.dtype).contiguous()).reshape(shp)
+
+
+class NormQuant(NamedTuple):
+    """What ``add_rms_norm_quant`` returns; ``h`` and ``y`` are None where they were not asked for."""
+    q: torch.Tensor  # float8_e4m3fn, as x
+    scale: torch.Tensor  # float32 [..., N / group]
+    h: Optional[torch.Tensor]  # x + residual, in x's type
+    y: Optional[torch.Tensor]  # the normalised row, in x's type
+
+
+def add_rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                       eps: float = 1e-6, group: int = 128, pow2_scale: bool = False,
+                       return_norm: bool = False) -> NormQuant:
+    """h = x + residual, y = rms_norm(h) * weight, and y in e4m3 with one scale for every ``group`` values:
+
+        scale = max(max |y|, 1e-4) / 448, or the next power of two (``pow2_scale``);  q = e4m3(y / scale)
+
+    the operand format of ``fp8_gemm`` for ``group=128``.  ``group=0``: one scale for each row; otherwise a power
+    of two from 16 to 512 that divides the row.  x [..., N] in bf16, fp16 or fp32 (N up to 65536) with weight [N]
+    and residual of its type.  Sums and norms are float32 throughout: the codes come from the y that was not
+    rounded to x's type (``rms_norm`` followed by ``act_quant`` rounds it in between).  ``h`` is returned if a
+    residual is given, ``y`` with ``return_norm``.  Rows that hold infinities or not-a-numbers give
+    not-a-number codes.  No gradient: inputs that require one are refused while gradients are on.
+    """
+    return NormQuant(*_native.ops().add_rms_norm_quant(x, weight, residual, eps, group, pow2_scale, return_norm))
