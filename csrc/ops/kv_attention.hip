@@ -28,6 +28,9 @@ constexpr int kThreads = kWaves * 64;
 constexpr int kTile = 64;  // keys of one wave's step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// The operands of the first product: Q's type, into which e4m3 widens exactly.  (The matrix cores' own e4m3 product
+// needs no widening, with Q split into e4m3 parts; but it aligns its summands in few bits: sums of 128 were off by up
+// to 2^-12 of the largest summand, which a softmax statistic may not be.)
 template <Type TYPE> struct Half;
 template <> struct Half<kBF16> {
   using X8 = bf16x8;
@@ -57,6 +60,9 @@ template <> struct Half<kF16> {
     return r.x;
   }
 };
+using Wide = Half<kBF16>;  // the second product's operands
+
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // results under 2^-126 are zero
 
 __device__ inline float across_groups_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -73,13 +79,22 @@ __device__ inline uint32_t nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0
 // the first n bytes of four
 __device__ inline uint32_t first_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
 
+// The keys of one tile: where this lane's K rows and V columns begin, and its 16 keys' scales.
+struct Place {
+  const uint8_t *k, *v;
+  float ks, vs;
+  bool there;  // whether the page of its 16 keys is in the pool
+};
+
 template <Type TYPE, int DC, int NR>
 __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a) {
   using T = typename Scalar<TYPE>::type;
+  constexpr int ROWS = 16 * NR, DT = 4 * DC;  // rows of the workgroup, 16-wide slices of the head
   using H = Half<TYPE>;
   using X8 = typename H::X8;
-  constexpr int ROWS = 16 * NR, DT = 4 * DC;  // rows of the workgroup, 16-wide slices of the head
-  __shared__ float o_lds[ROWS][DC * 64 + 4];
+  constexpr int PASSES = NR > 2 ? 2 : 1;  // the waves join in so many passes over the head
+  constexpr int PITCH = DC * 64 / PASSES + 4;
+  __shared__ float o_lds[kWaves][ROWS][PITCH];
   __shared__ float m_lds[kWaves][ROWS], l_lds[kWaves][ROWS];
 
   const Cache& c = a.cache;
@@ -93,6 +108,40 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   const int last = (row0 + ROWS < rows ? row0 + ROWS : rows) - 1;
   // one behind the last key that a row of this workgroup sees and the table can name
   const int end = min(past + last / per + 1, c.table_width << c.page_shift);
+  const int tiles = end > 0 ? (end + kTile - 1) / kTile : 0;
+  const int tile0 = int(int64_t(tiles) * split / a.splits) + wave;
+  const int tile1 = int(int64_t(tiles) * (split + 1) / a.splits);
+
+  const int* table = c.table + b * c.table_stride;
+  const int64_t head_bytes = int64_t(page) * c.wide;
+  const auto place_of = [&](int tile) {
+    // a group of keys behind the end reads the last page
+    const auto page_of = [&](int key, bool& there) {
+      const int id = table[(key < end ? key : end - 1) >> c.page_shift];
+      there = id >= 0 && id < c.pages;
+      return (there ? int64_t(id) : int64_t(0)) * c.heads + head;
+    };
+    Place p;
+    const int key_k = tile * kTile + 16 * (col >> 2), key_v = tile * kTile + 16 * grp;
+    const int64_t page_k = page_of(key_k, p.there), page_v = page_of(key_v, p.there);
+    p.k = c.k + page_k * head_bytes + int64_t((key_k & (page - 1)) + (col & 3)) * c.wide + 16 * grp;
+    p.v = c.v + page_v * head_bytes + int64_t(col) * page + (key_v & (page - 1));
+    p.ks = c.k_scale[page_v];
+    p.vs = c.v_scale[page_v];
+    return p;
+  };
+  u32x4 kx[4][DC], vx[DT];
+  const auto load_k = [&](const Place& p) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int k = 0; k < DC; ++k) kx[t][k] = *reinterpret_cast<const u32x4*>(p.k + 4 * t * c.wide + 64 * k);
+  };
+  Place at;
+  if (tile0 < tile1) {
+    at = place_of(tile0);
+    load_k(at);
+  }
 
   X8 q[NR][2 * DC];
   int pos[NR];
@@ -101,178 +150,182 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
     const int row = row0 + 16 * r + col, i = row / per, h = head * per + row % per;
     pos[r] = row < rows ? min(past + i, end - 1) : -1;
     const T* p = static_cast<const T*>(a.q) + b * a.stride_b + i * a.stride_t + h * a.stride_h;
+    const bool whole = row < rows && c.dim == c.wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 #pragma unroll
-    for (int k = 0; k < 2 * DC; ++k)
+    for (int k = 0; k < 2 * DC; ++k) {
+      const int d = 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
+      if (whole) {
+        q[r][k] = *reinterpret_cast<const X8*>(p + d);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int d = 64 * (k >> 1) + 16 * grp + 8 * (k & 1) + j;
-        q[r][k][j] = row < rows && d < c.dim ? p[d] : T(0.0f);
+        for (int j = 0; j < 8; ++j) q[r][k][j] = row < rows && d + j < c.dim ? p[d + j] : T(0.0f);
       }
+      // the scores' scale may be negative; its sign goes here, so that the largest product is the largest score
+      if (a.scale < 0.0f) q[r][k] = -q[r][k];
+    }
   }
+  const float to_log2 = fabsf(a.scale) * kLog2e;
   f32x4 o[NR][DT] = {};
   float m[NR], l[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
 
-  const int tiles = end > 0 ? (end + kTile - 1) / kTile : 0;
-  const int tile1 = int(int64_t(tiles) * (split + 1) / a.splits);
-  const int* table = c.table + b * c.table_stride;
-  const int64_t head_bytes = int64_t(page) * c.wide;
-  const float to_log2 = a.scale * kLog2e;
+  for (int tile = tile0; tile < tile1; tile += kWaves) {
+    const int key0 = tile * kTile, key_v = key0 + 16 * grp;
+    const Place now = at;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vx[d] = *reinterpret_cast<const u32x4*>(now.v + 16 * d * page);
+    const bool more = tile + kWaves < tile1;
+    if (more) at = place_of(tile + kWaves);
 
-  for (int tile = int(int64_t(tiles) * split / a.splits) + wave; tile < tile1; tile += kWaves) {
-    const int key0 = tile * kTile;
-    // the pages of the lane's K row and of its 16 keys; a group of keys behind the end reads the last page
-    const auto page_of = [&](int key, bool& there) {
-      const int id = table[(key < end ? key : end - 1) >> c.page_shift];
-      there = id >= 0 && id < c.pages;
-      return there ? int64_t(id) : int64_t(0);
-    };
-    bool there;
-    const int key_k = key0 + 16 * (col >> 2), key_v = key0 + 16 * grp;
-    const int64_t page_k = page_of(key_k, there) * c.heads + head;
-    const int64_t page_v = page_of(key_v, there) * c.heads + head;
-    const uint8_t* kp = c.k + page_k * head_bytes + int64_t((key_k & (page - 1)) + (col & 3)) * c.wide + 16 * grp;
-    const uint8_t* vp = c.v + page_v * head_bytes + int64_t(col) * page + (key_v & (page - 1));
-    const float ks = c.k_scale[page_v] * to_log2, vs = c.v_scale[page_v];
-    u32x4 kx[4][DC], vx[DT];
+    f32x4 s[NR][4] = {};
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int k = 0; k < DC; ++k) kx[t][k] = *reinterpret_cast<const u32x4*>(kp + 4 * t * c.wide + 64 * k);
+      for (int k = 0; k < 2 * DC; ++k) {
+        const u32x4 x = kx[t][k >> 1];
+        const X8 k8 = k & 1 ? H::widen(x.z, x.w) : H::widen(x.x, x.y);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vx[d] = *reinterpret_cast<const u32x4*>(vp + 16 * d * page);
+        for (int r = 0; r < NR; ++r) s[r][t] = H::mfma(k8, q[r][k], s[r][t]);
+      }
+    if (more) load_k(at);
 
-    // what the slots behind the sequence hold must not reach the product, not even times zero
-    if (key0 + kTile > end || !there) {
-      const int n = there ? end - key_v : 0;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vx[d][j] &= first_bytes(n - 4 * j);
-    }
-    const bool diagonal = key0 + kTile > past + row0 / per + 1;  // some row does not see some key
-    bool bad = false;
-    if (diagonal) {
+    // some row does not see some key, or a page is absent
+    const bool masked = key0 + kTile > min(past + row0 / per + 1, end) || __any(!now.there);
+    if (masked) {
+      const int n = now.there ? end - key_v : 0;
       uint32_t found = 0;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) found |= nan_bytes(vx[d][j]);
-      bad = __any(found != 0);
+        for (int j = 0; j < 4; ++j) {
+          vx[d][j] &= first_bytes(n - 4 * j);  // what lies behind the sequence must not count, not even times zero
+          found |= nan_bytes(vx[d][j]);
+        }
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!now.there || key_v + 4 * t + i > pos[r]) s[r][t][i] = -INFINITY;
+      if (__any(found != 0)) {
+        // a row that sees a not-a-number becomes one, a row that does not stays as it is: count the seen ones
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          uint32_t bad[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            bad[j] = nan_bytes(vx[d][j]) >> 7;  // 1 where not-a-number
+            vx[d][j] &= ~(bad[j] * 0xff);
+          }
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            f32x4 count = {};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              bf16x8 seen;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) seen[e] = __bf16(now.there && key_v + 8 * u + e <= pos[r] ? 1.0f : 0.0f);
+              count = Wide::mfma(Wide::widen(bad[2 * u] * 0x38, bad[2 * u + 1] * 0x38), seen, count);  // 0x38: 1.0
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[r][d][i] = count[i] > 0.0f ? NAN : o[r][d][i];
+          }
+        }
+      }
     }
 
+    const float vs = now.there ? now.vs : 0.0f;
+    bf16x8 hi[NR][2], lo[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      f32x4 s[4] = {};
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int k = 0; k < DC; ++k) {
-          s[t] = H::mfma(H::widen(kx[t][k].x, kx[t][k].y), q[r][2 * k], s[t]);
-          s[t] = H::mfma(H::widen(kx[t][k].z, kx[t][k].w), q[r][2 * k + 1], s[t]);
-        }
+      const float ks = fmaxf(now.ks * to_log2, 1e-30f);  // never zero: a hidden score stays -inf
       float top = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool seen = there && key_v + 4 * t + i <= pos[r];
-          s[t][i] = seen ? s[t][i] * ks : -INFINITY;
-          top = fmaxf(top, s[t][i]);
-        }
-      top = fmaxf(m[r], across_groups_max(top));
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float alpha = exp2f(m[r] - base);
-      m[r] = top;
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[r][t][i]);
+      top = across_groups_max(top * ks);
+      // The sums are relative to m.  It moves only when the scores outgrow it by more than 2^8: weights up to
+      // 2^8 lose nothing in bf16 and float32.
+      if (__any(top > m[r] + 8.0f)) {
+        const float next = fmaxf(m[r], top), alpha = next == -INFINITY ? 1.0f : exp2_of(m[r] - next);
+        m[r] = next;
+        l[r] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[r][d] *= alpha;
+      }
+      const float base = m[r] == -INFINITY ? 0.0f : m[r];
       float sum = 0.0f;
-      bf16x8 hi[2], lo[2];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = exp2f(s[t][i] - base);
+          const float p = exp2_of(fmaf(s[r][t][i], ks, -base));
           sum += p;
-          const float w = there ? p * vs : 0.0f;
-          hi[t >> 1][4 * (t & 1) + i] = __bf16(w);
-          if (TYPE == kF16) lo[t >> 1][4 * (t & 1) + i] = __bf16(w - float(__bf16(w)));
+          const float w = p * vs;
+          hi[r][t >> 1][4 * (t & 1) + i] = __bf16(w);
+          if (TYPE == kF16) lo[r][t >> 1][4 * (t & 1) + i] = __bf16(w - float(__bf16(w)));
         }
-      l[r] = l[r] * alpha + sum;
+      l[r] += sum;
+    }
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        o[r][d] *= alpha;
-        u32x4 x = vx[d];
-        if (bad) {
-          // a row that sees a not-a-number becomes one, a row that does not stays as it is: count the seen ones
-          bf16x8 seen[2];
-          f32x4 count = {};
+    for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) seen[e >> 3][e & 7] = __bf16(there && key_v + e <= pos[r] ? 1.0f : 0.0f);
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8 v = Wide::widen(vx[d][2 * u], vx[d][2 * u + 1]);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t n0 = nan_bytes(x[2 * u]) >> 7, n1 = nan_bytes(x[2 * u + 1]) >> 7;  // 1 where not-a-number
-            const bf16x8 is = Half<kBF16>::widen(n0 * 0x38, n1 * 0x38);                       // 0x38: 1.0
-            count = Half<kBF16>::mfma(is, seen[u], count);
-            x[2 * u] &= ~(n0 * 0xff);
-            x[2 * u + 1] &= ~(n1 * 0xff);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[r][d][i] = count[i] > 0.0f ? NAN : o[r][d][i];
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bf16x8 v8 = Half<kBF16>::widen(x[2 * u], x[2 * u + 1]);
-          o[r][d] = Half<kBF16>::mfma(v8, hi[u], o[r][d]);
-          if (TYPE == kF16) o[r][d] = Half<kBF16>::mfma(v8, lo[u], o[r][d]);
+        for (int r = 0; r < NR; ++r) {
+          o[r][d] = Wide::mfma(v, hi[r][u], o[r][d]);
+          if (TYPE == kF16) o[r][d] = Wide::mfma(v, lo[r][u], o[r][d]);
         }
       }
-    }
   }
 
-  // join the waves: the largest maximum, then the sums relative to it, one wave after the other
+  // join the waves: sums relative to the largest maximum
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     l[r] = across_groups_sum(l[r]);
     if (grp == 0) m_lds[wave][16 * r + col] = m[r], l_lds[wave][16 * r + col] = l[r];
   }
-  __syncthreads();
+  constexpr int WIDTH = DC * 64 / PASSES;
+  const int here = rows - row0 < ROWS ? rows - row0 : ROWS;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    float top = m_lds[0][16 * r + col];
+  for (int pass = 0; pass < PASSES; ++pass) {
+    if (pass) __syncthreads();
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][16 * r + col]);
-    const float f = exp2f(m[r] - (top == -INFINITY ? 0.0f : top));
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[r][d] *= f;
-  }
-  for (int w = 0; w < kWaves; ++w) {
-    if (wave == w) {
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          f32x4* p = reinterpret_cast<f32x4*>(&o_lds[16 * r + col][16 * d + 4 * grp]);
-          *p = w == 0 ? o[r][d] : *p + o[r][d];
-        }
-    }
+      for (int d = 0; d < DT / PASSES; ++d)
+        *reinterpret_cast<f32x4*>(&o_lds[wave][16 * r + col][16 * d + 4 * grp]) = o[r][pass * (DT / PASSES) + d];
     __syncthreads();
-  }
-
-  for (int i = threadIdx.x; i < ROWS * c.dim; i += kThreads) {
-    const int r = i / c.dim, d = i - r * c.dim, row = row0 + r;
-    if (row >= rows) break;
-    float top = m_lds[0][r], sum = 0.0f;
+    for (int i = threadIdx.x; i < here * (WIDTH / 4); i += kThreads) {
+      const int r = i / (WIDTH / 4), d4 = i % (WIDTH / 4) * 4, d0 = pass * WIDTH + d4, row = row0 + r;
+      float top = m_lds[0][r], sum = 0.0f;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][r]);
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][r]);
+      f32x4 v = {};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += l_lds[w][r] * exp2f(m_lds[w][r] - (top == -INFINITY ? 0.0f : top));
-    const int64_t at = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
-    if (a.splits == 1) {
-      static_cast<T*>(a.out)[at * c.dim + d] = T(sum == 0.0f ? 0.0f : o_lds[r][d] / sum);
-      if (d == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-    } else {
-      a.part_o[(at * a.splits + split) * c.dim + d] = o_lds[r][d];
-      if (d == 0) a.part_ml[(at * a.splits + split) * 2] = top, a.part_ml[(at * a.splits + split) * 2 + 1] = sum;
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = m_lds[w][r] == -INFINITY ? 0.0f : exp2_of(m_lds[w][r] - top);
+        sum += l_lds[w][r] * f;
+        v += *reinterpret_cast<const f32x4*>(&o_lds[w][r][d4]) * f;
+      }
+      const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
+      if (a.splits == 1) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d0 + j < c.dim) static_cast<T*>(a.out)[out * c.dim + d0 + j] = T(v[j] * inv);
+        if (d0 == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+      } else {
+        const int64_t part = out * a.splits + split;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d0 + j < c.dim) a.part_o[part * c.dim + d0 + j] = v[j];
+        if (d0 == 0) a.part_ml[part * 2] = top, a.part_ml[part * 2 + 1] = sum;
+      }
     }
   }
 }
@@ -289,7 +342,7 @@ __global__ __launch_bounds__(64) void kv_join_kernel(AttentionArgs a) {
   float sum = 0.0f, o[4] = {};
   for (int s = 0; s < a.splits; ++s) {
     if (ml[2 * s + 1] == 0.0f) continue;  // it had no keys
-    const float w = exp2f(ml[2 * s] - (top == -INFINITY ? 0.0f : top));
+    const float w = exp2_of(ml[2 * s] - (top == -INFINITY ? 0.0f : top));
     sum += ml[2 * s + 1] * w;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
