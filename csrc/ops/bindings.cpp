@@ -4,10 +4,12 @@
 // workspaces from torch's allocator on the current stream (so a call can be captured into a graph, and two calls
 // share no scratch memory) and hands plain argument blocks to the gfx950 kernels, or to their host forms for CPU
 // tensors.  Tensors of any device may be passed, whatever device is current.
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <sstream>
 #include <string>
 #include <vector>
@@ -27,14 +29,12 @@ std::string text(const A&... a) {
   return os.str();
 }
 
-template <typename... A>
-void need(bool ok, const A&... a) {
-  if (!ok) throw py::value_error(text(a...));
-}
-template <typename... A>
-void need_type(bool ok, const A&... a) {
-  if (!ok) throw py::type_error(text(a...));
-}
+// The message is put together only where the check fails.
+#define NEED_AS(error, ok, ...) \
+  do {                          \
+    if (!(ok)) throw error(text(__VA_ARGS__)); \
+  } while (0)
+#define NEED(ok, ...) NEED_AS(py::value_error, ok, __VA_ARGS__)
 
 // One call's tensors: all on the first one's device, none asking for a gradient.
 struct Call {
@@ -42,29 +42,29 @@ struct Call {
   c10::optional<c10::Device> device;
 
   void on(const Tensor& t, const char* arg) {
-    need(t.defined(), name, ": argument '", arg, "' is an undefined tensor");
+    NEED(t.defined(), name, ": argument '", arg, "' is an undefined tensor");
     if (!device) {
-      need(t.is_cpu() || t.is_cuda(), name, ": argument '", arg, "' must be a CPU or a ROCm (cuda) tensor, got ",
+      NEED(t.is_cpu() || t.is_cuda(), name, ": argument '", arg, "' must be a CPU or a ROCm (cuda) tensor, got ",
            t.device().str());
       device = t.device();
     }
-    need(t.device() == *device, name, ": argument '", arg, "' is on ", t.device().str(), ", expected ",
+    NEED(t.device() == *device, name, ": argument '", arg, "' is on ", t.device().str(), ", expected ",
          device->str());
     if (t.requires_grad() && at::GradMode::is_enabled())
       throw std::runtime_error(text(name, ": argument '", arg, "' requires a gradient, and the operator has none"));
   }
   void dims(const Tensor& t, const char* arg, int64_t n) const {
-    need(t.dim() == n, name, ": argument '", arg, "' has ", t.dim(), " dims, expected ", n);
+    NEED(t.dim() == n, name, ": argument '", arg, "' has ", t.dim(), " dims, expected ", n);
   }
   void size(const Tensor& t, const char* arg, int d, int64_t n) const {
-    need(t.size(d) == n, name, ": argument '", arg, "' dim ", d, " is ", t.size(d), ", expected ", n);
+    NEED(t.size(d) == n, name, ": argument '", arg, "' dim ", d, " is ", t.size(d), ", expected ", n);
   }
   void dtype(const Tensor& t, const char* arg, c10::ScalarType s) const {
-    need_type(t.scalar_type() == s, name, ": argument '", arg, "' has dtype ", c10::toString(t.scalar_type()),
+    NEED_AS(py::type_error, t.scalar_type() == s, name, ": argument '", arg, "' has dtype ", c10::toString(t.scalar_type()),
               ", expected ", c10::toString(s));
   }
   void contiguous(const Tensor& t, const char* arg) const {
-    need(t.is_contiguous(), name, ": argument '", arg, "' must be contiguous");
+    NEED(t.is_contiguous(), name, ": argument '", arg, "' must be contiguous");
   }
   tl_ops::Type type(const Tensor& t, const char* arg, bool f32) const {
     switch (t.scalar_type()) {
@@ -79,13 +79,20 @@ struct Call {
     }
   }
   bool cpu() const { return device->is_cpu(); }
+  // Memory of the current stream, straight from the device's allocator.
+  Tensor fresh(c10::IntArrayRef sizes, c10::ScalarType s) const {
+    if (cpu()) return at::empty(sizes, at::TensorOptions().dtype(s));
+    return at::detail::empty_cuda(sizes, s, *device, c10::nullopt);
+  }
   tl_ops::Stream stream() const { return c10::hip::getCurrentHIPStream(device->index()).stream(); }
 };
 
 Tensor last_dense(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
 // [..., n] as [rows, n] with dense rows
-Tensor rows_of(const Tensor& t, int64_t n) { return last_dense(t.reshape({t.numel() / n, n})); }
+Tensor rows_of(const Tensor& t, int64_t n) {
+  return last_dense(t.dim() == 2 ? t : t.reshape({t.numel() / n, n}));
+}
 
 // ------------------------------------------------------------------------------------------- norm
 
@@ -95,37 +102,37 @@ py::tuple add_rms_norm_quant(const Tensor& x, const Tensor& weight, const OptTen
   c.on(x, "x");
   c.on(weight, "weight");
   if (residual) c.on(*residual, "residual");
-  need(x.dim() >= 1, c.name, ": argument 'x' has 0 dims, expected 1 or more");
+  NEED(x.dim() >= 1, c.name, ": argument 'x' has 0 dims, expected 1 or more");
   const int64_t n = x.size(-1);
   tl_ops::NormQuantArgs a{};
   a.type = c.type(x, "x", true);
-  need(n >= 1 && n <= tl_ops::kNormMaxWidth, c.name, ": rows of ", n, " elements, expected 1 to ",
+  NEED(n >= 1 && n <= tl_ops::kNormMaxWidth, c.name, ": rows of ", n, " elements, expected 1 to ",
        tl_ops::kNormMaxWidth);
   c.dims(weight, "weight", 1);
   c.size(weight, "weight", 0, n);
   c.dtype(weight, "weight", x.scalar_type());
   if (residual) {
     c.dtype(*residual, "residual", x.scalar_type());
-    need(residual->sizes() == x.sizes(), c.name, ": residual ", residual->sizes(), " does not match x ", x.sizes());
+    NEED(residual->sizes() == x.sizes(), c.name, ": residual ", residual->sizes(), " does not match x ", x.sizes());
   }
-  need(group == 0 || (group >= 16 && group <= 512 && (group & (group - 1)) == 0), c.name, ": group is ", group,
+  NEED(group == 0 || (group >= 16 && group <= 512 && (group & (group - 1)) == 0), c.name, ": group is ", group,
        ", expected 0 (one scale for each row) or a power of two from 16 to 512");
-  need(group == 0 || n % group == 0, c.name, ": rows of ", n, " elements do not split into groups of ", group);
+  NEED(group == 0 || n % group == 0, c.name, ": rows of ", n, " elements do not split into groups of ", group);
 
   c10::DeviceGuard guard(*c.device);
   const Tensor x2 = rows_of(x, n), w = weight.contiguous(), r2 = residual ? rows_of(*residual, n) : Tensor();
   a.rows = x2.size(0);
-  need(a.rows <= INT32_MAX, c.name, ": ", a.rows, " rows, expected fewer than 2^31");
+  NEED(a.rows <= INT32_MAX, c.name, ": ", a.rows, " rows, expected fewer than 2^31");
   a.width = int(n);
   a.group = int(group ? group : n);
   a.eps = float(eps);
   a.pow2 = pow2;
   std::vector<int64_t> scales(x.sizes().begin(), x.sizes().end());
   scales.back() = n / a.group;
-  const Tensor q = at::empty(x.sizes(), x.options().dtype(c10::ScalarType::Float8_e4m3fn));
-  const Tensor s = at::empty(scales, x.options().dtype(c10::ScalarType::Float));
-  const Tensor h = residual ? at::empty(x.sizes(), x.options()) : Tensor();
-  const Tensor y = return_norm ? at::empty(x.sizes(), x.options()) : Tensor();
+  const Tensor q = c.fresh(x.sizes(), c10::ScalarType::Float8_e4m3fn);
+  const Tensor s = c.fresh(scales, c10::ScalarType::Float);
+  const Tensor h = residual ? c.fresh(x.sizes(), x.scalar_type()) : Tensor();
+  const Tensor y = return_norm ? c.fresh(x.sizes(), x.scalar_type()) : Tensor();
   a.x = x2.data_ptr();
   a.x_stride = x2.stride(0);
   a.weight = w.data_ptr();
@@ -154,13 +161,13 @@ tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& 
   c.dims(k, "cache.k", 4);
   c.dims(v, "cache.v", 4);
   const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2), wide = k.size(3);
-  need(pages >= 1 && pages <= INT32_MAX && heads >= 1 && heads <= 65535, c.name, ": a cache of ", pages, " pages and ",
-       heads, " heads");
-  need(page >= 16 && page <= 1024 && (page & (page - 1)) == 0, c.name, ": pages of ", page,
+  NEED(pages >= 1 && heads >= 1 && heads <= 65535 && pages * heads <= INT32_MAX, c.name, ": a cache of ", pages,
+       " pages and ", heads, " heads");
+  NEED(page >= 16 && page <= 1024 && (page & (page - 1)) == 0, c.name, ": pages of ", page,
        " tokens, expected a power of two from 16 to 1024");
-  need(wide >= 64 && wide <= 256 && wide % 64 == 0, c.name, ": cache.k is ", wide,
+  NEED(wide >= 64 && wide <= 256 && wide % 64 == 0, c.name, ": cache.k is ", wide,
        " wide, expected a multiple of 64 up to 256");
-  need(dim >= 1 && dim <= wide && dim > wide - 64, c.name, ": heads of ", dim, " in a cache that is ", wide, " wide");
+  NEED(dim >= 1 && dim <= wide && dim > wide - 64, c.name, ": heads of ", dim, " in a cache that is ", wide, " wide");
   for (int d = 0; d < 4; ++d) c.size(v, "cache.v", d, k.size(d < 2 ? d : 5 - d));
   const std::pair<const Tensor*, const char*> scales[] = {{&ks, "cache.k_scale"}, {&vs, "cache.v_scale"}};
   for (const auto& t : scales) {
@@ -170,13 +177,13 @@ tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& 
     c.size(*t.first, t.second, 1, heads);
   }
   for (int i = 0; i < 4; ++i) c.contiguous(*all[i].first, all[i].second);
-  need(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
+  NEED(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
        c.name, ": the cache must begin on a 16-byte boundary");
   c.dtype(table, "block_table", c10::ScalarType::Int);
   c.dims(table, "block_table", 2);
   c.size(table, "block_table", 0, batch);
-  need(table.size(1) <= 1 || table.stride(1) == 1, c.name, ": block_table's rows must be dense");
-  need(table.size(1) * page <= (int64_t(1) << 30), c.name, ": block_table holds ", table.size(1), " pages of ", page,
+  NEED(table.size(1) <= 1 || table.stride(1) == 1, c.name, ": block_table's rows must be dense");
+  NEED(table.size(1) * page <= (int64_t(1) << 30), c.name, ": block_table holds ", table.size(1), " pages of ", page,
        " tokens, expected at most 2^30 tokens");
   c.dtype(lengths, "lengths", c10::ScalarType::Int);
   c.dims(lengths, "lengths", 1);
@@ -208,12 +215,12 @@ void kv_cache_append(const Tensor& k, const Tensor& v, const Tensor& ks, const T
   tl_ops::AppendArgs a{};
   a.type = c.type(new_k, "k", true);
   c.dtype(new_v, "v", new_k.scalar_type());
-  need(new_v.sizes() == new_k.sizes(), c.name, ": v ", new_v.sizes(), " does not match k ", new_k.sizes());
+  NEED(new_v.sizes() == new_k.sizes(), c.name, ": v ", new_v.sizes(), " does not match k ", new_k.sizes());
   a.cache = cache_of(c, k, v, ks, vs, dim, table, lengths, new_k.size(0));
   c.size(new_k, "k", 2, a.cache.heads);
   c.size(new_k, "k", 3, dim);
-  need(new_k.size(0) <= 32767, c.name, ": ", new_k.size(0), " sequences, expected at most 32767");
-  need(new_k.size(1) <= (int64_t(1) << 19), c.name, ": ", new_k.size(1), " new tokens, expected at most 2^19");
+  NEED(new_k.size(0) <= 32767, c.name, ": ", new_k.size(0), " sequences, expected at most 32767");
+  NEED(new_k.size(1) <= (int64_t(1) << 19), c.name, ": ", new_k.size(1), " new tokens, expected at most 2^19");
   a.batch = int(new_k.size(0));
   a.new_tokens = int(new_k.size(1));
   c10::DeviceGuard guard(*c.device);
@@ -241,19 +248,18 @@ py::object kv_cache_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   a.cache = cache_of(c, k, v, ks, vs, dim, table, lengths, q.size(0));
   c.size(q, "q", 3, dim);
   const int64_t batch = q.size(0), tokens = q.size(1), heads = q.size(2);
-  need(heads >= 1 && heads % a.cache.heads == 0, c.name, ": ", heads, " query heads do not share ", a.cache.heads,
+  NEED(heads >= 1 && heads % a.cache.heads == 0, c.name, ": ", heads, " query heads do not share ", a.cache.heads,
        " key heads");
-  need(batch <= 65535, c.name, ": ", batch, " sequences, expected at most 65535");
-  need(tokens * heads <= (int64_t(1) << 27) && batch * tokens * heads <= INT32_MAX, c.name, ": ", batch, " x ", tokens,
+  NEED(batch <= 65535, c.name, ": ", batch, " sequences, expected at most 65535");
+  NEED(tokens * heads <= (int64_t(1) << 27) && batch * tokens * heads <= INT32_MAX, c.name, ": ", batch, " x ", tokens,
        " x ", heads, " query rows are too many for one call");
   a.batch = int(batch);
   a.new_tokens = int(tokens);
   a.heads = int(heads);
   a.scale = scale ? float(*scale) : 1.0f / std::sqrt(float(dim));
   c10::DeviceGuard guard(*c.device);
-  const Tensor q2 = last_dense(q), out = at::empty(q.sizes(), q.options());
-  const auto f32 = q.options().dtype(c10::ScalarType::Float);
-  const Tensor lse = return_lse ? at::empty({batch, tokens, heads}, f32) : Tensor();
+  const Tensor q2 = last_dense(q), out = c.fresh(q.sizes(), q.scalar_type());
+  const Tensor lse = return_lse ? c.fresh({batch, tokens, heads}, c10::ScalarType::Float) : Tensor();
   a.q = q2.data_ptr();
   a.stride_b = q2.stride(0);
   a.stride_t = q2.stride(1);
@@ -268,7 +274,7 @@ py::object kv_cache_attention(const Tensor& q, const Tensor& k, const Tensor& v,
     Tensor parts;  // freed on return: torch's allocator hands it out again behind this stream's work only
     if (a.splits > 1) {
       const int64_t n = batch * tokens * heads * a.splits;
-      parts = at::empty({n * (dim + 2)}, f32);
+      parts = c.fresh({n * (dim + 2)}, c10::ScalarType::Float);
       a.part_o = static_cast<float*>(parts.data_ptr());
       a.part_ml = a.part_o + n * dim;
     }
@@ -289,7 +295,7 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, int64_t take, 
   c.dims(scores, "scores", 2);
   c.dtype(scores, "scores", c10::ScalarType::Float);
   const int64_t batch = scores.size(0), beams = scores.size(1);
-  need(logits.dim() == 2 || logits.dim() == 3, c.name, ": argument 'logits' has ", logits.dim(),
+  NEED(logits.dim() == 2 || logits.dim() == 3, c.name, ": argument 'logits' has ", logits.dim(),
        " dims, expected 2 or 3");
   tl_ops::BeamArgs a{};
   a.type = c.type(logits, "logits", true);
@@ -300,22 +306,22 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, int64_t take, 
     c.size(logits, "logits", 0, batch * beams);
   }
   const int64_t vocab = logits.size(-1);
-  need(vocab >= 1 && vocab <= INT32_MAX - 1 && beams >= 1 && beams <= tl_ops::kBeamMaxBeams, c.name, ": ", beams,
+  NEED(vocab >= 1 && vocab <= INT32_MAX - 1 && beams >= 1 && beams <= tl_ops::kBeamMaxBeams, c.name, ": ", beams,
        " beams over ", vocab, " tokens, expected 1 to ", tl_ops::kBeamMaxBeams, " beams over at least one token");
-  need(take >= 1 && take <= tl_ops::kBeamMaxTake && take <= beams * vocab, c.name, ": take is ", take,
+  NEED(take >= 1 && take <= tl_ops::kBeamMaxTake && take <= beams * vocab, c.name, ": take is ", take,
        ", expected 1 to ", std::min<int64_t>(tl_ops::kBeamMaxTake, beams * vocab));
-  need(batch * beams <= 65535, c.name, ": ", batch * beams, " rows, expected at most 65535");
+  NEED(batch * beams <= 65535, c.name, ": ", batch * beams, " rows, expected at most 65535");
   if (finished) {
     c.dtype(*finished, "finished", c10::ScalarType::Bool);
-    need(finished->sizes() == scores.sizes(), c.name, ": finished ", finished->sizes(), " does not match scores ",
+    NEED(finished->sizes() == scores.sizes(), c.name, ": finished ", finished->sizes(), " does not match scores ",
          scores.sizes());
-    need(eos >= 0 && eos < vocab, c.name, ": eos_id is ", eos, ", expected one of the ", vocab, " tokens");
+    NEED(eos >= 0 && eos < vocab, c.name, ": eos_id is ", eos, ", expected one of the ", vocab, " tokens");
   }
   c10::DeviceGuard guard(*c.device);
   const Tensor x = rows_of(logits, vocab), sc = scores.contiguous(), fin = finished ? finished->contiguous() : Tensor();
-  const auto i64 = scores.options().dtype(c10::ScalarType::Long);
-  const Tensor out_scores = at::empty({batch, take}, scores.options()), out_parents = at::empty({batch, take}, i64),
-               out_tokens = at::empty({batch, take}, i64);
+  const Tensor out_scores = c.fresh({batch, take}, c10::ScalarType::Float),
+               out_parents = c.fresh({batch, take}, c10::ScalarType::Long),
+               out_tokens = c.fresh({batch, take}, c10::ScalarType::Long);
   a.logits = x.data_ptr();
   a.stride = x.stride(0);
   a.scores = static_cast<const float*>(sc.data_ptr());
@@ -332,10 +338,10 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, int64_t take, 
     tl_ops::beam_select_cpu(a);
   } else if (batch) {
     a.chunks = tl_ops::beam_select_chunks(batch * beams, a.vocab);
-    need(beams * a.chunks <= tl_ops::kBeamMaxLists, c.name, ": ", beams, " beams over ", vocab,
+    NEED(beams * a.chunks <= tl_ops::kBeamMaxLists, c.name, ": ", beams, " beams over ", vocab,
          " tokens are too many for one call");
     const int64_t n = batch * beams * a.chunks;
-    const Tensor parts = at::empty({n * (take + 1)}, i64);
+    const Tensor parts = c.fresh({n * (take + 1)}, c10::ScalarType::Long);
     a.part_list = static_cast<uint64_t*>(parts.data_ptr());
     a.part_stat = reinterpret_cast<float*>(a.part_list + n * take);
     tl_ops::beam_select_hip(a, c.stream());
@@ -350,23 +356,28 @@ void reorder_states(const std::vector<Tensor>& states, const Tensor& parents, co
   c.dims(parents, "parents", 2);
   c.contiguous(parents, "parents");
   const int64_t batch = parents.size(0), beams = parents.size(1), rows = batch * beams;
-  need(beams >= 1 && beams <= tl_ops::kReorderMaxBeams, c.name, ": ", beams, " beams, expected 1 to ",
+  NEED(beams >= 1 && beams <= tl_ops::kReorderMaxBeams, c.name, ": ", beams, " beams, expected 1 to ",
        tl_ops::kReorderMaxBeams);
-  need(batch <= 65535, c.name, ": ", batch, " sequences, expected at most 65535");
-  need(!length || *length >= 0, c.name, ": length is ", length.value_or(0), ", expected 0 or more");
+  NEED(batch <= 65535, c.name, ": ", batch, " sequences, expected at most 65535");
+  NEED(!length || *length >= 0, c.name, ": length is ", length.value_or(0), ", expected 0 or more");
   std::vector<tl_ops::ReorderState> moved;
   for (const Tensor& t : states) {
     c.on(t, "states");
-    need(t.dim() >= (length ? 2 : 1), c.name, ": a state has ", t.dim(), " dims, expected ", length ? 2 : 1,
+    NEED(t.dim() >= (length ? 2 : 1), c.name, ": a state has ", t.dim(), " dims, expected ", length ? 2 : 1,
          " or more");
-    need(t.size(0) == rows, c.name, ": a state has ", t.size(0), " rows, expected ", batch, " x ", beams);
-    need(!length || *length <= t.size(1), c.name, ": length is ", length.value_or(0), ", and a state has ", t.size(1));
+    NEED(t.size(0) == rows, c.name, ": a state has ", t.size(0), " rows, expected ", batch, " x ", beams);
+    NEED(!length || *length <= t.size(1), c.name, ": length is ", length.value_or(0), ", and a state has ", t.size(1));
     if (t.numel() == 0) continue;
-    const Tensor row = length ? t.select(0, 0).narrow(0, 0, *length) : t.select(0, 0);
-    need(row.is_contiguous(), c.name, ": what moves of a state's row must be contiguous");
-    const int64_t bytes = row.numel() * int64_t(t.element_size()), stride = t.stride(0) * int64_t(t.element_size());
+    // what moves of a row: its elements, dense from the row's beginning
+    int64_t moves = 1;
+    for (int64_t d = t.dim() - 1; d >= 1; --d) {
+      const int64_t n = d == 1 && length ? *length : t.size(d);
+      NEED(n <= 1 || t.stride(d) == moves, c.name, ": what moves of a state's row must be contiguous");
+      moves *= n;
+    }
+    const int64_t bytes = moves * int64_t(t.element_size()), stride = t.stride(0) * int64_t(t.element_size());
     if (bytes == 0) continue;
-    need(rows == 1 || stride >= bytes, c.name, ": a state's rows overlap");
+    NEED(rows == 1 || stride >= bytes, c.name, ": a state's rows overlap");
     moved.push_back({static_cast<uint8_t*>(t.data_ptr()), stride, bytes});
   }
   // No byte may be moved twice.  In the order of their addresses, two states that share a range must be columns of
@@ -377,7 +388,7 @@ void reorder_states(const std::vector<Tensor>& states, const Tensor& parents, co
   for (size_t i = 0; i < sorted.size(); ++i)
     for (size_t j = i + 1; j < sorted.size() && sorted[j].data < end(sorted[i]); ++j) {
       const int64_t off = (sorted[j].data - sorted[i].data) % std::max<int64_t>(sorted[i].stride, 1);
-      need(rows > 1 && sorted[i].stride == sorted[j].stride && off >= sorted[i].bytes &&
+      NEED(rows > 1 && sorted[i].stride == sorted[j].stride && off >= sorted[i].bytes &&
                off + sorted[j].bytes <= sorted[i].stride,
            c.name, ": two states share memory");
     }

@@ -18,6 +18,8 @@
 //
 // The waves of a workgroup take tiles in turn and join in LDS; `splits` workgroups share a long key axis and
 // kv_join_kernel joins them.
+#include <type_traits>
+
 #include "device.h"
 
 namespace tl_ops {
@@ -64,13 +66,14 @@ using Wide = Half<kBF16>;  // the second product's operands
 
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }  // results under 2^-126 are zero
 
-__device__ inline float across_groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ inline float across_groups_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+// The lanes that hold a row's keys are 16 and 32 apart; a swap of a register with itself leaves both halves of each
+// pair in both lanes, without a trip through LDS.
+template <typename F>
+__device__ inline float across_groups(float v, F f) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // e4m3 bytes that are not-a-number (0x7f, 0xff): bit 7 of each such byte
@@ -79,14 +82,122 @@ __device__ inline uint32_t nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0
 // the first n bytes of four
 __device__ inline uint32_t first_bytes(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
 
-// The keys of one tile: where this lane's K rows and V columns begin, and its 16 keys' scales.
+// One row's Q as operands of the first product; the scores' scale may be negative, and its sign goes here, so that
+// the largest product is the largest score.
+template <Type TYPE, int DC>
+__device__ inline void load_q(const AttentionArgs& a, int b, int head, int row, int rows, int grp,
+                              typename Half<TYPE>::X8 (&q)[2 * DC]) {
+  using T = typename Scalar<TYPE>::type;
+  using X8 = typename Half<TYPE>::X8;
+  const Cache& c = a.cache;
+  const int per = a.heads / c.heads, i = row / per, h = head * per + row % per;
+  const T* p = static_cast<const T*>(a.q) + b * a.stride_b + i * a.stride_t + h * a.stride_h;
+  const bool whole = row < rows && c.dim == c.wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+#pragma unroll
+  for (int k = 0; k < 2 * DC; ++k) {
+    const int d = 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
+    if (whole) {
+      q[k] = *reinterpret_cast<const X8*>(p + d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[k][j] = row < rows && d + j < c.dim ? p[d + j] : T(0.0f);
+    }
+    if (a.scale < 0.0f) q[k] = -q[k];
+  }
+}
+
+// Scores of keys behind the row's position, or of a page that is not there, become -inf.
+__device__ inline void hide(f32x4 (&s)[4], bool there, int key, int pos) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!there || key + 4 * t + i > pos) s[t][i] = -INFINITY;
+}
+
+// A row that sees one of the not-a-numbers that `is` marks becomes one, a row that does not stays as it is.
+__device__ inline void poison(bf16x8 is, bool there, int key, int pos, f32x4& o) {
+  bf16x8 seen;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) seen[e] = __bf16(there && key + e <= pos ? 1.0f : 0.0f);
+  const f32x4 count = Wide::mfma(is, seen, f32x4{});
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = count[i] > 0.0f ? NAN : o[i];
+}
+
+// The weights of 16 scores of each of NR rows (in units of 1 / ks), with V's scale, as operands of the second
+// product; a page that is not `there` has none.  The sums are relative to m, which moves only when the scores outgrow it by more than 2^8: weights up to
+// 2^8 lose nothing in bf16 and float32.
+template <Type TYPE, int NR, int DT>
+__device__ inline void softmax_step(const f32x4 (&s)[NR][4], float ks, float vs, bool there, float (&m)[NR],
+                                    float (&l)[NR], f32x4 (&o)[NR][DT], bf16x8 (&hi)[NR][2], bf16x8 (&lo)[NR][2]) {
+  float top[NR];
+  bool grown = false;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    top[r] = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], s[r][t][i]);
+    top[r] = across_groups(there ? top[r] * ks : -INFINITY, Max());
+    grown |= top[r] > m[r] + 8.0f;
+  }
+  if (__any(grown)) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float next = fmaxf(m[r], top[r]), alpha = next == -INFINITY ? 1.0f : exp2_of(m[r] - next);
+      m[r] = next;
+      l[r] *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[r][d] *= alpha;
+    }
+  }
+  // V's scale goes into the exponent; it is taken as 2^-100 where it is less
+  vs = fmaxf(vs, 0x1p-100f);
+  const float log_vs = __builtin_amdgcn_logf(vs), inv_vs = 1.0f / vs;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const float base = there ? log_vs - (m[r] == -INFINITY ? 0.0f : m[r]) : -INFINITY;
+    float sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = exp2_of(fmaf(s[r][t][i], ks, base));
+        sum += w;
+        hi[r][t >> 1][4 * (t & 1) + i] = __bf16(w);
+        if (TYPE == kF16) lo[r][t >> 1][4 * (t & 1) + i] = __bf16(w - float(__bf16(w)));
+      }
+    l[r] += sum * inv_vs;
+  }
+}
+
+// Values at .. at + 3 of a row of `dim` (at % 4 == 0); at once where every row begins on such a boundary.
+template <typename T>
+__device__ inline void store4(T* row, f32x4 v, int at, int dim) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  if (dim % 4 == 0) {
+    if (at < dim) *reinterpret_cast<T4*>(row + at) = T4{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i < dim) row[at + i] = T(v[i]);
+  }
+}
+
+// The pages of a lane's K row and of its 16 keys in one tile, and where they are.  Pages of 64 tokens and more hold
+// WHOLE tiles: then both are one page for all lanes, and its id, address and scales stay in scalar registers.
+struct Pages {
+  int k, v;
+};
 struct Place {
   const uint8_t *k, *v;
   float ks, vs;
   bool there;  // whether the page of its 16 keys is in the pool
 };
 
-template <Type TYPE, int DC, int NR>
+template <Type TYPE, int DC, int NR, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a) {
   using T = typename Scalar<TYPE>::type;
   constexpr int ROWS = 16 * NR, DT = 4 * DC;  // rows of the workgroup, 16-wide slices of the head
@@ -98,7 +209,8 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   __shared__ float m_lds[kWaves][ROWS], l_lds[kWaves][ROWS];
 
   const Cache& c = a.cache;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
   const int split = blockIdx.y, b = blockIdx.z;
   const int head = int(blockIdx.x) % c.heads, row0 = int(blockIdx.x) / c.heads * ROWS;
   const int per = a.heads / c.heads, rows = a.new_tokens * per;  // query heads of a key head
@@ -113,19 +225,22 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   const int tile1 = int(int64_t(tiles) * (split + 1) / a.splits);
 
   const int* table = c.table + b * c.table_stride;
-  const int64_t head_bytes = int64_t(page) * c.wide;
-  const auto place_of = [&](int tile) {
+  const uint32_t head_bytes = uint32_t(page) * c.wide;
+  const auto pages_of = [&](int tile) {
     // a group of keys behind the end reads the last page
-    const auto page_of = [&](int key, bool& there) {
-      const int id = table[(key < end ? key : end - 1) >> c.page_shift];
-      there = id >= 0 && id < c.pages;
-      return (there ? int64_t(id) : int64_t(0)) * c.heads + head;
-    };
-    Place p;
+    const auto page_of = [&](int key) { return table[(key < end ? key : end - 1) >> c.page_shift]; };
+    if (WHOLE) return Pages{page_of(tile * kTile), page_of(tile * kTile)};
+    return Pages{page_of(tile * kTile + 16 * (col >> 2)), page_of(tile * kTile + 16 * grp)};
+  };
+  const auto place_of = [&](int tile, Pages id) {
+    const auto in_pool = [&](int i) { return i >= 0 && i < c.pages; };
     const int key_k = tile * kTile + 16 * (col >> 2), key_v = tile * kTile + 16 * grp;
-    const int64_t page_k = page_of(key_k, p.there), page_v = page_of(key_v, p.there);
-    p.k = c.k + page_k * head_bytes + int64_t((key_k & (page - 1)) + (col & 3)) * c.wide + 16 * grp;
-    p.v = c.v + page_v * head_bytes + int64_t(col) * page + (key_v & (page - 1));
+    const uint32_t page_k = uint32_t(in_pool(id.k) ? id.k : 0) * c.heads + head;
+    const uint32_t page_v = uint32_t(in_pool(id.v) ? id.v : 0) * c.heads + head;
+    Place p;
+    p.there = in_pool(id.v);
+    p.k = c.k + uint64_t(page_k) * head_bytes + ((key_k & (page - 1)) + (col & 3)) * c.wide + 16 * grp;
+    p.v = c.v + uint64_t(page_v) * head_bytes + (key_v & (page - 1));
     p.ks = c.k_scale[page_v];
     p.vs = c.v_scale[page_v];
     return p;
@@ -137,9 +252,15 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
 #pragma unroll
       for (int k = 0; k < DC; ++k) kx[t][k] = *reinterpret_cast<const u32x4*>(p.k + 4 * t * c.wide + 64 * k);
   };
-  Place at;
+  // What a tile needs is asked for a tile ahead (its pages' ids two ahead), and V behind K: no wait is for a load
+  // that has just been issued.  Behind the last tile the loads repeat it.
+  const auto ahead = [&](int tile) { return tile < tile1 ? tile : tile1 - 1; };
+  Place at{};
+  Pages next{};
   if (tile0 < tile1) {
-    at = place_of(tile0);
+    const Pages first = pages_of(tile0);
+    next = pages_of(ahead(tile0 + kWaves));
+    at = place_of(tile0, first);
     load_k(at);
   }
 
@@ -147,22 +268,9 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   int pos[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    const int row = row0 + 16 * r + col, i = row / per, h = head * per + row % per;
-    pos[r] = row < rows ? min(past + i, end - 1) : -1;
-    const T* p = static_cast<const T*>(a.q) + b * a.stride_b + i * a.stride_t + h * a.stride_h;
-    const bool whole = row < rows && c.dim == c.wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-#pragma unroll
-    for (int k = 0; k < 2 * DC; ++k) {
-      const int d = 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
-      if (whole) {
-        q[r][k] = *reinterpret_cast<const X8*>(p + d);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[r][k][j] = row < rows && d + j < c.dim ? p[d + j] : T(0.0f);
-      }
-      // the scores' scale may be negative; its sign goes here, so that the largest product is the largest score
-      if (a.scale < 0.0f) q[r][k] = -q[r][k];
-    }
+    const int row = row0 + 16 * r + col;
+    pos[r] = row < rows ? min(past + row / per, end - 1) : -1;
+    load_q<TYPE, DC>(a, b, head, row, rows, grp, q[r]);
   }
   const float to_log2 = fabsf(a.scale) * kLog2e;
   f32x4 o[NR][DT] = {};
@@ -174,9 +282,10 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
     const int key0 = tile * kTile, key_v = key0 + 16 * grp;
     const Place now = at;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vx[d] = *reinterpret_cast<const u32x4*>(now.v + 16 * d * page);
-    const bool more = tile + kWaves < tile1;
-    if (more) at = place_of(tile + kWaves);
+    for (int d = 0; d < DT; ++d)  // a padded row is not read: another one stands in, its result is not written
+      vx[d] = *reinterpret_cast<const u32x4*>(now.v + (16 * d + col < c.dim ? 16 * d + col : c.dim - 1) * page);
+    at = place_of(ahead(tile + kWaves), next);
+    next = pages_of(ahead(tile + 2 * kWaves));
 
     f32x4 s[NR][4] = {};
 #pragma unroll
@@ -188,7 +297,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
 #pragma unroll
         for (int r = 0; r < NR; ++r) s[r][t] = H::mfma(k8, q[r][k], s[r][t]);
       }
-    if (more) load_k(at);
+    load_k(at);
 
     // some row does not see some key, or a page is absent
     const bool masked = key0 + kTile > min(past + row0 / per + 1, end) || __any(!now.there);
@@ -203,73 +312,26 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
           found |= nan_bytes(vx[d][j]);
         }
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!now.there || key_v + 4 * t + i > pos[r]) s[r][t][i] = -INFINITY;
+      for (int r = 0; r < NR; ++r) hide(s[r], now.there, key_v, pos[r]);
       if (__any(found != 0)) {
-        // a row that sees a not-a-number becomes one, a row that does not stays as it is: count the seen ones
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          uint32_t bad[4];
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            bad[j] = nan_bytes(vx[d][j]) >> 7;  // 1 where not-a-number
-            vx[d][j] &= ~(bad[j] * 0xff);
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t n0 = nan_bytes(vx[d][2 * u]) >> 7, n1 = nan_bytes(vx[d][2 * u + 1]) >> 7;
+            vx[d][2 * u] &= ~(n0 * 0xff);
+            vx[d][2 * u + 1] &= ~(n1 * 0xff);
+            const bf16x8 is = Wide::widen(n0 * 0x38, n1 * 0x38);  // 0x38: 1.0
+#pragma unroll
+            for (int r = 0; r < NR; ++r) poison(is, now.there, key_v + 8 * u, pos[r], o[r][d]);
           }
-#pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            f32x4 count = {};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              bf16x8 seen;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) seen[e] = __bf16(now.there && key_v + 8 * u + e <= pos[r] ? 1.0f : 0.0f);
-              count = Wide::mfma(Wide::widen(bad[2 * u] * 0x38, bad[2 * u + 1] * 0x38), seen, count);  // 0x38: 1.0
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[r][d][i] = count[i] > 0.0f ? NAN : o[r][d][i];
-          }
-        }
       }
     }
 
+    const float ks = fmaxf(now.ks * to_log2, 1e-30f);  // never zero: a hidden score stays -inf
     const float vs = now.there ? now.vs : 0.0f;
     bf16x8 hi[NR][2], lo[NR][2];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      const float ks = fmaxf(now.ks * to_log2, 1e-30f);  // never zero: a hidden score stays -inf
-      float top = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[r][t][i]);
-      top = across_groups_max(top * ks);
-      // The sums are relative to m.  It moves only when the scores outgrow it by more than 2^8: weights up to
-      // 2^8 lose nothing in bf16 and float32.
-      if (__any(top > m[r] + 8.0f)) {
-        const float next = fmaxf(m[r], top), alpha = next == -INFINITY ? 1.0f : exp2_of(m[r] - next);
-        m[r] = next;
-        l[r] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] *= alpha;
-      }
-      const float base = m[r] == -INFINITY ? 0.0f : m[r];
-      float sum = 0.0f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = exp2_of(fmaf(s[r][t][i], ks, -base));
-          sum += p;
-          const float w = p * vs;
-          hi[r][t >> 1][4 * (t & 1) + i] = __bf16(w);
-          if (TYPE == kF16) lo[r][t >> 1][4 * (t & 1) + i] = __bf16(w - float(__bf16(w)));
-        }
-      l[r] += sum;
-    }
+    softmax_step<TYPE, NR, DT>(s, ks, vs, now.there, m, l, o, hi, lo);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -286,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   // join the waves: sums relative to the largest maximum
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    l[r] = across_groups_sum(l[r]);
+    l[r] = across_groups(l[r], Add());
     if (grp == 0) m_lds[wave][16 * r + col] = m[r], l_lds[wave][16 * r + col] = l[r];
   }
   constexpr int WIDTH = DC * 64 / PASSES;
@@ -315,62 +377,329 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
       const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
       if (a.splits == 1) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d0 + j < c.dim) static_cast<T*>(a.out)[out * c.dim + d0 + j] = T(v[j] * inv);
+        store4(static_cast<T*>(a.out) + out * c.dim, v * inv, d0, c.dim);
         if (d0 == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
         const int64_t part = out * a.splits + split;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (d0 + j < c.dim) a.part_o[part * c.dim + d0 + j] = v[j];
+        store4(a.part_o + part * c.dim, v, d0, c.dim);
         if (d0 == 0) a.part_ml[part * 2] = top, a.part_ml[part * 2 + 1] = sum;
       }
     }
   }
 }
 
-// One wave joins one row's parts: weights 2^(m_s - max m), the sum of the weighted sums below.
-template <Type TYPE>
+// The form for many rows (chunks of prompts): the matrix cores bound it, so the keys of a step are widened once for
+// all rows.  A workgroup holds 128 rows, 32 to a wave; waves 0-3 take the even tiles, waves 4-7 the odd ones, two
+// waves to a SIMD so that one's softmax runs beside the other's products.  Each step's two tiles lie in LDS as the
+// operands that the products read (16 bytes a lane, in lane order: no bank conflict), in two buffers: the next step
+// is loaded during the products and written behind them, with one barrier a step.
+constexpr int kChunkWaves = 8, kChunkThreads = kChunkWaves * 64, kChunkRows = 128;
+
+template <Type TYPE, int DC, bool WHOLE>
+__global__ __launch_bounds__(kChunkThreads, 2) void kv_attention_chunk_kernel(AttentionArgs a) {
+  using T = typename Scalar<TYPE>::type;
+  using H = Half<TYPE>;
+  using X8 = typename H::X8;
+  constexpr int DT = 4 * DC, NR = 2, PITCH = DC * 64 + 4;
+  struct Tile {
+    X8 k[4][2 * DC][64];
+    bf16x8 v[DT][2][64];
+  };
+  struct Scales {
+    float ks, vs;
+    int there;
+  };
+  union Lds {
+    Tile tile[2][2];
+    float o[kChunkRows][PITCH];
+  };
+  __shared__ Lds lds;
+  __shared__ Scales scales[2][2][4];
+  // V's not-a-numbers go as zeros into the product and reach the rows that see them by `poison`: whether what a wave
+  // wrote holds any (a byte for each), and where (bit e: key 16 grp + e of the lane).  Only where some row does not
+  // see all of the tile: elsewhere they may spread by themselves
+  __shared__ uint32_t nan[2][2];
+  __shared__ uint16_t nan_marks[2][2][DT][64];
+  __shared__ float m_lds[kChunkRows], l_lds[kChunkRows];
+
+  const Cache& c = a.cache;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int part = wave >> 2, mine = wave & 3;  // the tile of a step, and what of it this wave loads
+  const int split = blockIdx.y, b = blockIdx.z;
+  const int head = int(blockIdx.x) % c.heads, row0 = int(blockIdx.x) / c.heads * kChunkRows;
+  const int per = a.heads / c.heads, rows = a.new_tokens * per;
+  const int page = 1 << c.page_shift;
+  const int past = max(c.lengths[b], 0) - a.new_tokens;
+  const int last = min(row0 + kChunkRows, rows) - 1;
+  const int end = min(past + last / per + 1, c.table_width << c.page_shift);
+  const int steps = end > 0 ? (end + 2 * kTile - 1) / (2 * kTile) : 0;
+  const int step0 = int(int64_t(steps) * split / a.splits), step1 = int(int64_t(steps) * (split + 1) / a.splits);
+  const int* table = c.table + b * c.table_stride;
+  const uint32_t head_bytes = uint32_t(page) * c.wide;
+
+  // This wave's share of a tile: K rows of slice `mine`, V's slices `mine`, `mine` + 4, ..  A step's loads are issued
+  // a step before they are written to LDS (its pages' ids another step before); behind the last step they repeat it.
+  u32x4 kx[DC], vx[DC];
+  Scales sc{};
+  bool k_there = true;
+  const auto ahead = [&](int step) { return step < step1 ? step : step1 - 1; };
+  const auto pages_of = [&](int step) {
+    const int key0 = (2 * ahead(step) + part) * kTile;
+    // a group of keys behind the end reads the last page
+    const auto page_of = [&](int key) { return table[(key < end ? key : end - 1) >> c.page_shift]; };
+    if (WHOLE) return Pages{page_of(key0), page_of(key0)};
+    return Pages{page_of(key0 + 16 * (col >> 2)), page_of(key0 + 16 * grp)};
+  };
+  const auto load = [&](int step, Pages id) {
+    const int key0 = (2 * ahead(step) + part) * kTile, key_k = key0 + 16 * (col >> 2), key_v = key0 + 16 * grp;
+    const auto in_pool = [&](int i) { return i >= 0 && i < c.pages; };
+    const uint32_t page_k = uint32_t(in_pool(id.k) ? id.k : 0) * c.heads + head;
+    const uint32_t page_v = uint32_t(in_pool(id.v) ? id.v : 0) * c.heads + head;
+    const uint8_t* kp = c.k + uint64_t(page_k) * head_bytes + ((key_k & (page - 1)) + (col & 3) + 4 * mine) * c.wide +
+                        16 * grp;
+    const uint8_t* vp = c.v + uint64_t(page_v) * head_bytes + (16 * mine + col) * page + (key_v & (page - 1));
+#pragma unroll
+    for (int k = 0; k < DC; ++k) kx[k] = *reinterpret_cast<const u32x4*>(kp + 64 * k);
+#pragma unroll
+    for (int d = 0; d < DC; ++d) vx[d] = *reinterpret_cast<const u32x4*>(vp + 64 * d * page);
+    sc = {c.k_scale[page_v], c.v_scale[page_v], in_pool(id.v)};
+    k_there = in_pool(id.k);
+  };
+  const auto write = [&](int step, int buf) {
+    if (__any(!k_there)) {  // the scores of a page that is not there stay finite, and its weights become zero
+#pragma unroll
+      for (int k = 0; k < DC; ++k) kx[k] = k_there ? kx[k] : u32x4{};
+    }
+#pragma unroll
+    for (int k = 0; k < DC; ++k) {
+      lds.tile[buf][part].k[mine][2 * k][lane] = H::widen(kx[k].x, kx[k].y);
+      lds.tile[buf][part].k[mine][2 * k + 1][lane] = H::widen(kx[k].z, kx[k].w);
+    }
+    const int key0 = (2 * ahead(step) + part) * kTile;
+    if (key0 + kTile > end || __any(!sc.there)) {
+      // what lies behind the sequence must not count, not even times zero
+      const int n = sc.there ? end - key0 - 16 * grp : 0;
+#pragma unroll
+      for (int d = 0; d < DC; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vx[d][j] &= first_bytes(n - 4 * j);
+    }
+    uint32_t found = 0;
+    if (key0 + kTile > past + row0 / per + 1) {
+#pragma unroll
+      for (int d = 0; d < DC; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) found |= nan_bytes(vx[d][j]);
+      found = __any(found != 0);
+    }
+    if (lane == 0) reinterpret_cast<uint8_t*>(&nan[buf][part])[mine] = uint8_t(found);
+    if (mine == 0 && col == 0) scales[buf][part][grp] = sc;
+#pragma unroll
+    for (int d = 0; d < DC; ++d) {
+      if (found) {
+        uint32_t marks = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t n = nan_bytes(vx[d][j]) >> 7;
+          marks |= ((n | n >> 7 | n >> 14 | n >> 21) & 15) << (4 * j);
+          vx[d][j] &= ~(n * 0xff);
+        }
+        nan_marks[buf][part][mine + 4 * d][lane] = uint16_t(marks);
+      }
+      lds.tile[buf][part].v[mine + 4 * d][0][lane] = Wide::widen(vx[d].x, vx[d].y);
+      lds.tile[buf][part].v[mine + 4 * d][1][lane] = Wide::widen(vx[d].z, vx[d].w);
+    }
+  };
+
+  X8 q[NR][2 * DC];
+  int pos[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int row = row0 + 32 * mine + 16 * r + col;
+    pos[r] = row < rows ? min(past + row / per, end - 1) : -1;
+    load_q<TYPE, DC>(a, b, head, row, rows, grp, q[r]);
+  }
+  const float to_log2 = fabsf(a.scale) * kLog2e;
+  f32x4 o[NR][DT] = {};
+  float m[NR], l[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+
+  Pages next{};
+  if (step0 < step1) {
+    load(step0, pages_of(step0));
+    next = pages_of(step0 + 1);
+    write(step0, step0 & 1);
+    load(step0 + 1, next);
+    next = pages_of(step0 + 2);
+  }
+  __syncthreads();
+  const auto run = [&](int step, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;  // whether some row does not see some key
+    const int buf = step & 1, key_v = (2 * step + part) * kTile + 16 * grp;
+    const Tile& t = lds.tile[buf][part];
+    f32x4 s[NR][4] = {};
+#pragma unroll
+    for (int k = 0; k < 2 * DC; ++k)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        const X8 k8 = t.k[kt][k][lane];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r][kt] = H::mfma(k8, q[r][k], s[r][kt]);
+      }
+    const Scales now = scales[buf][part][grp];
+    if (MASKED) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) hide(s[r], now.there, key_v, pos[r]);
+    }
+    bf16x8 hi[NR][2], lo[NR][2];
+    softmax_step<TYPE, NR, DT>(s, fmaxf(now.ks * to_log2, 1e-30f), now.vs, now.there, m, l, o, hi, lo);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bf16x8 v8 = t.v[d][u][lane];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          o[r][d] = Wide::mfma(v8, hi[r][u], o[r][d]);
+          if (TYPE == kF16) o[r][d] = Wide::mfma(v8, lo[r][u], o[r][d]);
+        }
+      }
+    const uint32_t bad = MASKED ? __builtin_amdgcn_readfirstlane(nan[buf][part]) : 0;
+    if (bad) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        if (!(bad >> (8 * (d & 3)) & 1)) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t marks = nan_marks[buf][part][d][lane] >> (8 * u);
+          bf16x8 is;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) is[e] = __bf16(marks >> e & 1 ? 1.0f : 0.0f);
+#pragma unroll
+          for (int r = 0; r < NR; ++r) poison(is, now.there, key_v + 8 * u, pos[r], o[r][d]);
+        }
+      }
+    }
+    write(step + 1, buf ^ 1);
+    load(step + 2, next);
+    next = pages_of(step + 3);
+    __syncthreads();
+  };
+  // the steps whose keys all rows see
+  const int clean = max(step0, min(step1, min(past + row0 / per + 1, end) / (2 * kTile)));
+  int step = step0;
+  for (; step < clean; ++step) run(step, std::false_type());
+  for (; step < step1; ++step) run(step, std::true_type());
+
+  // waves 4-7 hand their sums to waves 0-3, which hold the same rows
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    l[r] = across_groups(l[r], Add());
+    const int at = 32 * mine + 16 * r + col;
+    if (part == 1) {
+      if (grp == 0) m_lds[at] = m[r], l_lds[at] = l[r];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&lds.o[at][16 * d + 4 * grp]) = o[r][d];
+    }
+  }
+  __syncthreads();
+  if (part == 1) return;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int at = 32 * mine + 16 * r + col, row = row0 + at;
+    if (row >= rows) continue;
+    const float top = fmaxf(m[r], m_lds[at]);
+    const float f0 = m[r] == -INFINITY ? 0.0f : exp2_of(m[r] - top);
+    const float f1 = m_lds[at] == -INFINITY ? 0.0f : exp2_of(m_lds[at] - top);
+    const float sum = l[r] * f0 + l_lds[at] * f1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
+    const int64_t part_at = out * a.splits + split;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const f32x4 v = o[r][d] * f0 + *reinterpret_cast<const f32x4*>(&lds.o[at][16 * d + 4 * grp]) * f1;
+      if (a.splits == 1)
+        store4(static_cast<T*>(a.out) + out * c.dim, v * inv, 16 * d + 4 * grp, c.dim);
+      else
+        store4(a.part_o + part_at * c.dim, v, 16 * d + 4 * grp, c.dim);
+    }
+    if (grp == 0) {
+      if (a.splits > 1)
+        a.part_ml[part_at * 2] = top, a.part_ml[part_at * 2 + 1] = sum;
+      else if (a.lse)
+        a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    }
+  }
+}
+
+constexpr int kJoinMost = 128;  // parts of one row
+
+// One wave joins one row's parts: weights 2^(m_s - max m), the sum of the weighted sums below.  A lane holds the
+// statistics of parts lane and lane + 64, and the loads of eight parts are in flight together.
+template <Type TYPE, int DC>
 __global__ __launch_bounds__(64) void kv_join_kernel(AttentionArgs a) {
   using T = typename Scalar<TYPE>::type;
   const int64_t at = blockIdx.x;
-  const int lane = threadIdx.x, dim = a.cache.dim;
-  const float* ml = a.part_ml + at * a.splits * 2;
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
-  float sum = 0.0f, o[4] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    if (ml[2 * s + 1] == 0.0f) continue;  // it had no keys
-    const float w = exp2_of(ml[2 * s] - (top == -INFINITY ? 0.0f : top));
-    sum += ml[2 * s + 1] * w;
+  const int lane = threadIdx.x, dim = a.cache.dim, splits = a.splits;
+  const float* ml = a.part_ml + at * splits * 2;
+  const float* part = a.part_o + at * splits * dim;
+  float m[2], l[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (64 * j + lane < dim) o[j] += w * a.part_o[(at * a.splits + s) * dim + 64 * j + lane];
+  for (int j = 0; j < 2; ++j) {
+    const int s = 64 * j + lane;
+    m[j] = s < splits ? ml[2 * s] : -INFINITY;
+    l[j] = s < splits ? ml[2 * s + 1] : 0.0f;
+  }
+  const float top = wave_reduce(fmaxf(m[0], m[1]), Max());
+#pragma unroll
+  for (int j = 0; j < 2; ++j) m[j] = m[j] == -INFINITY ? 0.0f : exp2_of(m[j] - top);  // a part without keys: 0
+  const float sum = wave_reduce(l[0] * m[0] + l[1] * m[1], Add());
+  float o[DC] = {};
+  constexpr int BATCH = 8;  // parts whose loads are in flight together; behind the last one they repeat it
+  for (int s0 = 0; s0 < splits; s0 += BATCH) {
+    float v[BATCH][DC];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+      for (int j = 0; j < DC; ++j)
+        v[k][j] = part[int64_t(min(s0 + k, splits - 1)) * dim + min(64 * j + lane, dim - 1)];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int s = s0 + k;
+      const float w = s < splits ? __shfl(s < 64 ? m[0] : m[1], s & 63) : 0.0f;  // a part without keys holds zeros
+#pragma unroll
+      for (int j = 0; j < DC; ++j) o[j] += s < splits ? w * v[k][j] : 0.0f;
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < DC; ++j)
     if (64 * j + lane < dim)
       static_cast<T*>(a.out)[at * dim + 64 * j + lane] = T(sum == 0.0f ? 0.0f : o[j] / sum);
   if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-template <Type TYPE, int DC, int NR>
-void launch_rows(const AttentionArgs& a, Stream s) {
-  const int rows = a.new_tokens * (a.heads / a.cache.heads);
-  const dim3 grid(unsigned(a.cache.heads * ceil_div(rows, 16 * NR)), a.splits, a.batch);
-  launch(kv_attention_kernel<TYPE, DC, NR>, grid, kThreads, a, s, "kv_cache_attention");
-  if (a.splits > 1)
-    launch(kv_join_kernel<TYPE>, dim3(unsigned(a.batch * a.new_tokens * a.heads)), 64, a, s, "kv_cache_attention");
-}
+// The rows of a workgroup: as few 16-row tiles as hold a key head's rows, or 128 where they are many (heads over 128
+// wide: 32, their tiles do not fit LDS twice).
+int rows_of(int rows, int wide) { return rows <= 16 ? 16 : rows <= 32 || wide > 128 ? 32 : kChunkRows; }
 
-// Rows that a workgroup takes: as few 16-row tiles as hold a key head's rows, up to what the registers hold.
 template <Type TYPE, int DC>
 void launch_dim(const AttentionArgs& a, Stream s) {
-  const int rows = a.new_tokens * (a.heads / a.cache.heads);
-  if (rows <= 16) return launch_rows<TYPE, DC, 1>(a, s);
-  if (rows <= 32 || DC > 2) return launch_rows<TYPE, DC, 2>(a, s);
-  if constexpr (DC <= 2) launch_rows<TYPE, DC, 4>(a, s);
+  const int rows = a.new_tokens * (a.heads / a.cache.heads), tile = rows_of(rows, a.cache.wide);
+  const dim3 grid(unsigned(a.cache.heads * ceil_div(rows, tile)), a.splits, a.batch);
+  const bool whole = 1 << a.cache.page_shift >= kTile;
+  const char* what = "kv_cache_attention";
+  if (tile == 16)
+    launch(whole ? kv_attention_kernel<TYPE, DC, 1, true> : kv_attention_kernel<TYPE, DC, 1, false>, grid, kThreads, a,
+           s, what);
+  else if (tile == 32)
+    launch(whole ? kv_attention_kernel<TYPE, DC, 2, true> : kv_attention_kernel<TYPE, DC, 2, false>, grid, kThreads, a,
+           s, what);
+  else if constexpr (DC <= 2)
+    launch(whole ? kv_attention_chunk_kernel<TYPE, DC, true> : kv_attention_chunk_kernel<TYPE, DC, false>, grid,
+           kChunkThreads, a, s, what);
+  if (a.splits > 1)
+    launch(kv_join_kernel<TYPE, DC>, dim3(unsigned(a.batch * a.new_tokens * a.heads)), 64, a, s, what);
 }
 
 template <Type TYPE>
@@ -385,13 +714,16 @@ void launch_type(const AttentionArgs& a, Stream s) {
 
 }  // namespace
 
+// One workgroup for each of the 256 CUs, and no less than 128 keys (two waves' tiles) for each.  Measured (us, heads of
+// 128, one new token, 32 on 8 heads), by parts of the key axis:
+//   1 x 8192 keys: 1 part 47, 8 13.9, 32 11.3, 64 13.7;      1 x 65536: 1 344, 16 35, 32 29, 64 32
+//   4 x 8192: 1 48, 4 21, 8 17, 32 22;                       32 x 8192: 1 82, 4 80, 16 107
 int kv_attention_splits(int batch, int new_tokens, int heads, int kv_heads, int wide, int64_t longest) {
-  const int rows = new_tokens * (heads / kv_heads), tile = rows <= 16 ? 16 : rows <= 32 || wide > 128 ? 32 : 64;
-  const int64_t groups = int64_t(batch) * kv_heads * ceil_div(rows, tile);
-  const int64_t most = ceil_div(longest, kTile * kWaves);  // a tile for every wave
-  int64_t want = ceil_div(1024, groups);
-  if (want > most) want = most;
-  return int(want < 1 ? 1 : want > 128 ? 128 : want);
+  const int rows = new_tokens * (heads / kv_heads);
+  const int64_t groups = int64_t(batch) * kv_heads * ceil_div(rows, rows_of(rows, wide));
+  int64_t parts = ceil_div(256, groups);
+  if (parts > ceil_div(longest, 2 * kTile)) parts = ceil_div(longest, 2 * kTile);
+  return int(parts < 1 ? 1 : parts > kJoinMost ? kJoinMost : parts);
 }
 
 void kv_attention_hip(const AttentionArgs& a, Stream s) {

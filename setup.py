@@ -44,7 +44,7 @@ ops = CppExtension(
     include_dirs=[os.path.join(ROCM, "include")],
     define_macros=[("__HIP_PLATFORM_AMD__", "1"), ("USE_ROCM", "1")],
     library_dirs=[os.path.join(ROCM, "lib")],
-    libraries=["amdhip64", "c10_hip"],
+    libraries=["amdhip64", "c10_hip", "torch_hip"],
     extra_compile_args=["-O2", "-std=c++17", "-fvisibility=hidden", "-Wno-unused-function"],
 )
 

@@ -36,4 +36,4 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, length
     0 .. beams - 1 leaves its beam as it is; at most 32 beams).  ``length``: only the first ``length`` entries of
     the states' second dimension move (the filled part of a cache).  What moves of a row must be contiguous, and
     no two states may share memory."""
-    _native.ops().reorder_states(list(states), parents, length)
+    _native.ops().reorder_states(states, parents, length)
