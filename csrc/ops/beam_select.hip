@@ -2,20 +2,27 @@
 //
 //   value[k, t] = score[k] + x[k, t] - logsumexp_t x[k, :];  largest first, ties to the lowest k * vocab + t
 //
-// Two launches, the logits are read once.  beam_scan_kernel: a workgroup holds one chunk of a row in registers and
-// writes its softmax statistics (maximum, sum of exponentials) and its `take` best logits in order, each as one
-// 64-bit key (logit's order in the upper half, ~token in the lower), so that ties go to the lowest token by
-// themselves.  Within a row the values have the logits' order, whatever the logarithm rounds to.
-// beam_merge_kernel: a workgroup per sequence joins the statistics, forms the values of the heads of all lists in
-// float64 (where two beams' values tie only if they are equal) and takes the best head `take` times.
+// Two launches; the logits are read once, and what is sorted is only what can win.
+//
+// beam_scan_kernel: a workgroup holds one chunk of a row in registers.  Its waves write the chunk's softmax
+// statistics (maximum, sum of exponentials), and the workgroup its `take` best logits in order, each as one 64-bit
+// key (the logit's order in the upper half, ~token in the lower), so that ties go to the lowest token by themselves.
+// If q lanes of a wave hold a logit of at least T, the chunk's q best are no less: with T the `take`-th largest of
+// the lanes' maxima, found bit by bit with one ballot each, few logits reach T.  Those go to LDS, and each finds its
+// place by counting the larger ones.
+// beam_merge_kernel: a workgroup per sequence joins the statistics and does the same with the lists' values, which
+// are float64: there two beams' values tie only where they are equal, and within a beam they have the logits' order.
+//
+// Where ties let too many candidates through (a constant row, say), the best one is taken `take` times instead.
 #include "device.h"
 
 namespace tl_ops {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kPer = 16;  // logits of a thread
-constexpr int kChunk = kThreads * kPer;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
+constexpr int kKept = 512;        // candidates of a chunk that LDS takes
+constexpr int kMergeKept = 2048;  // and of a sequence
 
 // The order of floats as that of unsigned integers; -0 counts as 0.
 __device__ inline uint32_t order_of(float x) {
@@ -24,6 +31,21 @@ __device__ inline uint32_t order_of(float x) {
 }
 __device__ inline float from_order(uint32_t k) {
   return __uint_as_float(k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
+}
+// The upper half of a double's order: a <= b gives order_of(a) <= order_of(b).
+__device__ inline uint32_t order_of(double x) {
+  const uint32_t u = uint32_t(__double2hiint(x + 0.0));
+  return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+
+// A value that at least `want` of the wave's lanes reach (the largest one, up to its last BITS left out).
+template <int BITS>
+__device__ inline uint32_t reached_by(uint32_t key, int want) {
+  uint32_t t = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit >= 1u << BITS; bit >>= 1)
+    if (__popcll(__ballot(key >= (t | bit))) >= want) t |= bit;
+  return t;
 }
 
 __device__ inline uint64_t wave_max(uint64_t v) {
@@ -34,55 +56,126 @@ __device__ inline uint64_t wave_max(uint64_t v) {
   }
   return v;
 }
+__device__ inline double wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
 
-template <Type TYPE>
+// A slot of `count` for every lane that keeps something, in lane order within the wave.
+__device__ inline int slot_for(bool keep, int* count) {
+  const uint64_t mask = __ballot(keep);
+  if (mask == 0) return 0;
+  const int lane = threadIdx.x & 63, first = __ffsll((unsigned long long)mask) - 1;
+  int base = 0;
+  if (lane == first) base = atomicAdd(count, __popcll(mask));
+  base = __shfl(base, first);
+  return base + int(__builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0)));
+}
+
+template <Type TYPE, int PER>
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamArgs a) {
   using T = typename Scalar<TYPE>::type;
-  __shared__ float f_lds[2][kThreads / 64];
-  __shared__ uint64_t best_lds[2][kThreads / 64];
-  const int tid = threadIdx.x, chunk = blockIdx.x;
+  constexpr int VEC = 16 / sizeof(T), VECS = PER / VEC, CHUNK = kThreads * PER;
+  __shared__ uint32_t t_lds[kWaves];
+  __shared__ uint64_t best_lds[2][kWaves];
+  __shared__ uint64_t kept[kKept];
+  __shared__ int count;
+  const int tid = threadIdx.x, wave = tid >> 6, chunk = blockIdx.x;
   const int64_t row = blockIdx.y;
-  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-  const int begin = int(int64_t(a.vocab) * chunk / a.chunks), end = int(int64_t(a.vocab) * (chunk + 1) / a.chunks);
-  float v[kPer];
+  const int begin = chunk * CHUNK, left = a.vocab - begin;  // tokens from the chunk on
+  const T* x = static_cast<const T*>(a.logits) + row * a.stride + begin;
+  if (tid == 0) count = 0;
+
+  // vector i of the thread: tokens at(i, 0) .. at(i, VEC - 1) of the chunk
+  const auto at = [&](int i, int e) { return (i * kThreads + tid) * VEC + e; };
+  float v[PER];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    if (at(i, VEC) <= left) {
+      T r[VEC];
+      __builtin_memcpy(r, x + at(i, 0), 16);  // rows begin anywhere
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = float(r[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = at(i, e) < left ? float(x[at(i, e)]) : -INFINITY;
+    }
+  }
   float top = -INFINITY;
   bool nan = false;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int t = begin + i * kThreads + tid;
-    v[i] = t < end ? float(x[t]) : -INFINITY;
-    nan |= v[i] != v[i];
-    top = fmaxf(top, v[i]);
+  for (int j = 0; j < PER; ++j) {
+    nan |= v[j] != v[j];
+    top = fmaxf(top, v[j]);
   }
-  top = block_reduce<kThreads>(top, f_lds[0], Max());
+  // the lane's largest key; 0 (less than any logit's) where it has no logit at all
+  const uint32_t mine = at(0, 0) < left ? order_of(top) : 0;
+  const uint32_t t = reached_by<12>(mine, a.take < 64 ? a.take : 64);
+  if ((tid & 63) == 0) t_lds[wave] = t;
+  top = wave_reduce(top, Max());
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) sum += begin + i * kThreads + tid < end ? expf(v[i] - top) : 0.0f;
-  sum = block_reduce<kThreads>(nan ? NAN : sum, f_lds[1], Add());
-  const int64_t at = row * a.chunks + chunk;
-  if (tid == 0) a.part_stat[2 * at] = top, a.part_stat[2 * at + 1] = top == -INFINITY ? 0.0f : sum;
-
-  uint64_t key[kPer], mine = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int t = begin + i * kThreads + tid;
-    key[i] = t < end ? uint64_t(order_of(v[i])) << 32 | uint32_t(~t) : 0;
-    mine = key[i] > mine ? key[i] : mine;
+  for (int j = 0; j < PER; ++j)
+    sum += top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v[j] - top) * 1.4426950408889634f);
+  sum = wave_reduce(nan ? NAN : sum, Add());
+  const int64_t list = row * a.chunks + chunk;
+  if ((tid & 63) == 0) {
+    float* stat = a.part_stat + (list * kWaves + wave) * 2;
+    stat[0] = top;
+    stat[1] = sum;
   }
-  for (int n = 0; n < a.take; ++n) {
-    uint64_t best = wave_max(mine);
-    if ((tid & 63) == 0) best_lds[n & 1][tid >> 6] = best;
+  __syncthreads();
+  uint32_t limit = 1;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) limit = t_lds[w] > limit ? t_lds[w] : limit;
+
+  const auto key_of = [&](int j) -> uint64_t {
+    const int token = at(j / VEC, j % VEC);
+    return token < left ? uint64_t(order_of(v[j])) << 32 | uint32_t(~(begin + token)) : 0;
+  };
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const uint64_t key = key_of(j);
+    const bool keep = uint32_t(key >> 32) >= limit;
+    if (__any(keep)) {
+      const int s = slot_for(keep, &count);
+      if (keep && s < kKept) kept[s] = key;
+    }
+  }
+  __syncthreads();
+  const int n = count;
+  uint64_t* out = a.part_list + list * a.take;
+  if (n <= kKept) {
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t key = kept[i];
+      int place = 0;
+      for (int j = 0; j < n; ++j) place += kept[j] > key;
+      if (place < a.take) out[place] = key;
+    }
+    for (int i = n + tid; i < a.take; i += kThreads) out[i] = 0;  // the chunk has no more
+    return;
+  }
+  uint64_t taken = ~0ull, best_of = 0;  // what the thread has left: its keys below the last one taken
+  const auto look = [&] {
+    best_of = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint64_t key = key_of(j);
+      if (key < taken && key > best_of) best_of = key;
+    }
+  };
+  look();
+  for (int k = 0; k < a.take; ++k) {
+    uint64_t best = wave_max(best_of);
+    if ((tid & 63) == 0) best_lds[k & 1][wave] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w) best = best_lds[n & 1][w] > best ? best_lds[n & 1][w] : best;
-    if (tid == 0) a.part_list[at * a.take + n] = best;  // 0: the chunk has no more
-    if (mine == best && best) {
-      mine = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (key[i] == best) key[i] = 0;
-        mine = key[i] > mine ? key[i] : mine;
-      }
+    for (int w = 0; w < kWaves; ++w) best = best_lds[k & 1][w] > best ? best_lds[k & 1][w] : best;
+    if (tid == 0) out[k] = best;
+    if (best_of == best && best) {
+      taken = best;
+      look();
     }
   }
 }
@@ -98,29 +191,37 @@ __device__ inline Candidate shuffle(const Candidate& c, int m) {
   return {__shfl_xor(c.value, m), (int64_t)__shfl_xor((long long)c.at, m)};
 }
 
-__global__ __launch_bounds__(kThreads) void beam_merge_kernel(BeamArgs a) {
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   __shared__ double lse_lds[kBeamMaxBeams];
-  __shared__ Candidate best_lds[2][kThreads / 64];
-  const int tid = threadIdx.x;
+  __shared__ Candidate kept[kMergeKept];
+  __shared__ Candidate best_lds[2][kMergeWaves];
+  __shared__ uint32_t t_lds[kMergeWaves];
+  __shared__ int count;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
   const double inf = INFINITY;
-  for (int k = tid; k < a.beams; k += kThreads) {
-    const float* stat = a.part_stat + (b * a.beams + k) * a.chunks * 2;
+  if (tid == 0) count = 0;
+  for (int k = wave; k < a.beams; k += kMergeWaves) {
+    const int n = a.chunks * kWaves;
+    const float* stat = a.part_stat + (b * a.beams + k) * n * 2;
     float top = -INFINITY;
-    for (int c = 0; c < a.chunks; ++c) top = fmaxf(top, stat[2 * c]);
-    double sum = 0.0;
-    for (int c = 0; c < a.chunks; ++c) sum += double(stat[2 * c + 1]) * exp(double(stat[2 * c]) - double(top));
-    lse_lds[k] = double(top) + log(sum);
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, stat[2 * i]);
+    top = wave_reduce(top, Max());
+    double sum = 0.0;  // not-a-number where a wave's is, or where the maximum is infinite: such a beam is dead
+    for (int i = lane; i < n; i += 64)
+      sum += double(stat[2 * i + 1]) * double(__builtin_amdgcn_exp2f((stat[2 * i] - top) * 1.4426950408889634f));
+    sum = wave_sum(sum);
+    if (lane == 0) lse_lds[k] = double(top) + log(sum);
   }
   __syncthreads();
 
   // List j belongs to beam j / chunks.  A beam without a finite score or logsumexp has only -inf to offer, a
   // finished one its eos token and -inf: their tokens are counted off by the beam's first list.
   const int lists = a.beams * a.chunks;
-  const auto head = [&](int j, int nth) -> Candidate {
+  const auto candidate = [&](int j, int nth) -> Candidate {
     const int k = j / a.chunks, c = j - k * a.chunks;
     const int64_t none = INT64_MAX, first = int64_t(k) * a.vocab;
-    if (nth >= a.take) return {-inf, none};
+    if (j >= lists || nth >= a.take) return {-inf, none};
     const float score = a.scores[b * a.beams + k];
     const double lse = lse_lds[k];
     const bool live = fabsf(score) < INFINITY, done = a.finished && a.finished[b * a.beams + k];
@@ -138,43 +239,78 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(BeamArgs a) {
     const double x = from_order(uint32_t(key >> 32));
     return {double(score) + (x - lse), first + uint32_t(~uint32_t(key))};
   };
-  Candidate mine{-inf, INT64_MAX};
-  int mine_list = -1;
-  // a list's position is the number of its candidates that won so far; kept by the thread that owns it
-  constexpr int kOwn = kBeamMaxLists / kThreads;
-  int taken[kOwn];
+  const auto order = [&](const Candidate& c) { return c.at == INT64_MAX ? 0u : order_of(c.value); };
+
+  // If q lists' candidates number j (from 0) reach T, the best q (j + 1) do: T is such that this is `take`.
+  const int lanes = lists < 64 ? lists : 64, nth = (a.take - 1) / lanes, q = (a.take + nth) / (nth + 1);
+  if (wave * 64 < lists) {
+    const uint32_t t = reached_by<0>(order(candidate(tid, nth)), q);
+    if (lane == 0) t_lds[wave] = t;
+  } else if (lane == 0) {
+    t_lds[wave] = 0;
+  }
+  __syncthreads();
+  uint32_t limit = 1;
+#pragma unroll
+  for (int w = 0; w < kMergeWaves; ++w) limit = t_lds[w] > limit ? t_lds[w] : limit;
+  // lists are in order: each is read up to its first candidate below T
+  for (int j0 = 0; j0 < lists; j0 += kMergeThreads) {
+    bool open = j0 + tid < lists;
+    for (int i = 0; i < a.take; ++i) {
+      Candidate c{-inf, INT64_MAX};
+      if (open) c = candidate(j0 + tid, i);
+      open = open && order(c) >= limit;
+      if (!__any(open)) break;
+      const int s = slot_for(open, &count);
+      if (open && s < kMergeKept) kept[s] = c;
+    }
+  }
+  __syncthreads();
+  const auto write = [&](int place, const Candidate& c) {
+    a.out_scores[b * a.take + place] = float(c.value);
+    a.out_parents[b * a.take + place] = c.at / a.vocab;
+    a.out_tokens[b * a.take + place] = c.at % a.vocab;
+  };
+  const int n = count;
+  if (n <= kMergeKept) {
+    for (int i = tid; i < n; i += kMergeThreads) {
+      const Candidate c = kept[i];
+      int place = 0;
+      for (int j = 0; j < n; ++j) place += before(kept[j], c);
+      if (place < a.take) write(place, c);
+    }
+    return;
+  }
+  // The best head of all lists, `take` times; a list's position is kept by the thread that owns it.
+  constexpr int kOwn = kBeamMaxLists / kMergeThreads;
+  uint8_t taken[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) taken[i] = 0;
+  Candidate mine{-inf, INT64_MAX};
+  int mine_list = -1;
   const auto look = [&] {
     mine = {-inf, INT64_MAX};
     mine_list = -1;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int j = i * kThreads + tid;
-      if (j < lists) {
-        const Candidate h = head(j, taken[i]);
-        if (before(h, mine)) mine = h, mine_list = i;
-      }
+      const Candidate h = candidate(i * kMergeThreads + tid, taken[i]);
+      if (before(h, mine)) mine = h, mine_list = i;
     }
   };
   look();
-  for (int n = 0; n < a.take; ++n) {
+  for (int k = 0; k < a.take; ++k) {
     Candidate best = mine;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
       const Candidate other = shuffle(best, m);
       if (before(other, best)) best = other;
     }
-    if ((tid & 63) == 0) best_lds[n & 1][tid >> 6] = best;
+    if (lane == 0) best_lds[k & 1][wave] = best;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; ++w)
-      if (before(best_lds[n & 1][w], best)) best = best_lds[n & 1][w];
-    if (tid == 0) {
-      a.out_scores[b * a.take + n] = float(best.value);
-      a.out_parents[b * a.take + n] = best.at / a.vocab;
-      a.out_tokens[b * a.take + n] = best.at % a.vocab;
-    }
+    for (int w = 0; w < kMergeWaves; ++w)
+      if (before(best_lds[k & 1][w], best)) best = best_lds[k & 1][w];
+    if (tid == 0) write(k, best);
     if (mine_list >= 0 && mine.at == best.at) {
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) taken[i] += i == mine_list;
@@ -183,18 +319,33 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(BeamArgs a) {
   }
 }
 
+// Logits of a thread: 16, or 64 where a row would have more than 64 chunks.
+int per_thread(int vocab) { return vocab <= 64 * 16 * kThreads ? 16 : 64; }
+
+template <Type TYPE>
+void launch_scan(const BeamArgs& a, Stream s) {
+  const dim3 grid(a.chunks, unsigned(a.batch * a.beams));
+  launch(per_thread(a.vocab) == 16 ? beam_scan_kernel<TYPE, 16> : beam_scan_kernel<TYPE, 64>, grid, kThreads, a, s,
+         "beam_select");
+}
+
 }  // namespace
 
-int beam_select_chunks(int64_t, int vocab) { return int(ceil_div(vocab, kChunk)); }
+int beam_select_chunks(int vocab) { return int(ceil_div(vocab, per_thread(vocab) * kThreads)); }
 
-void beam_select_hip(const BeamArgs& a, Stream s) {
+int64_t beam_select_scratch(int64_t rows, int chunks, int take) { return rows * chunks * (take + kWaves); }
+
+void beam_select_hip(BeamArgs a, uint64_t* scratch, Stream s) {
   if (a.batch == 0) return;
-  const dim3 grid(a.chunks, unsigned(a.batch * a.beams));
-  const auto scan = a.type == kF32   ? beam_scan_kernel<kF32>
-                    : a.type == kF16 ? beam_scan_kernel<kF16>
-                                     : beam_scan_kernel<kBF16>;
-  launch(scan, grid, kThreads, a, s, "beam_select");
-  launch(beam_merge_kernel, dim3(unsigned(a.batch)), kThreads, a, s, "beam_select");
+  a.part_list = scratch;
+  a.part_stat = reinterpret_cast<float*>(scratch + a.batch * a.beams * a.chunks * a.take);
+  if (a.type == kF32)
+    launch_scan<kF32>(a, s);
+  else if (a.type == kF16)
+    launch_scan<kF16>(a, s);
+  else
+    launch_scan<kBF16>(a, s);
+  launch(beam_merge_kernel, dim3(unsigned(a.batch)), kMergeThreads, a, s, "beam_select");
 }
 
 }  // namespace tl_ops

@@ -306,8 +306,9 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, int64_t take, 
     c.size(logits, "logits", 0, batch * beams);
   }
   const int64_t vocab = logits.size(-1);
-  NEED(vocab >= 1 && vocab <= INT32_MAX - 1 && beams >= 1 && beams <= tl_ops::kBeamMaxBeams, c.name, ": ", beams,
-       " beams over ", vocab, " tokens, expected 1 to ", tl_ops::kBeamMaxBeams, " beams over at least one token");
+  NEED(vocab >= 1 && vocab <= tl_ops::kBeamMaxVocab && beams >= 1 && beams <= tl_ops::kBeamMaxBeams, c.name, ": ",
+       beams, " beams over ", vocab, " tokens, expected 1 to ", tl_ops::kBeamMaxBeams, " beams over 1 to ",
+       tl_ops::kBeamMaxVocab, " tokens");
   NEED(take >= 1 && take <= tl_ops::kBeamMaxTake && take <= beams * vocab, c.name, ": take is ", take,
        ", expected 1 to ", std::min<int64_t>(tl_ops::kBeamMaxTake, beams * vocab));
   NEED(batch * beams <= 65535, c.name, ": ", batch * beams, " rows, expected at most 65535");
@@ -337,14 +338,10 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, int64_t take, 
   if (c.cpu()) {
     tl_ops::beam_select_cpu(a);
   } else if (batch) {
-    a.chunks = tl_ops::beam_select_chunks(batch * beams, a.vocab);
-    NEED(beams * a.chunks <= tl_ops::kBeamMaxLists, c.name, ": ", beams, " beams over ", vocab,
-         " tokens are too many for one call");
-    const int64_t n = batch * beams * a.chunks;
-    const Tensor parts = c.fresh({n * (take + 1)}, c10::ScalarType::Long);
-    a.part_list = static_cast<uint64_t*>(parts.data_ptr());
-    a.part_stat = reinterpret_cast<float*>(a.part_list + n * take);
-    tl_ops::beam_select_hip(a, c.stream());
+    a.chunks = tl_ops::beam_select_chunks(a.vocab);
+    const Tensor parts = c.fresh({tl_ops::beam_select_scratch(batch * beams, a.chunks, a.take)},
+                                 c10::ScalarType::Long);
+    tl_ops::beam_select_hip(a, static_cast<uint64_t*>(parts.data_ptr()), c.stream());
   }
   return py::make_tuple(out_scores, out_parents, out_tokens);
 }

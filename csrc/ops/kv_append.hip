@@ -10,8 +10,6 @@
 namespace tl_ops {
 namespace {
 
-constexpr int kThreads = 256;
-
 // Where a workgroup's new tokens go: slots [slot0, slot0 + n) of the page, token `first` onwards.
 struct Span {
   int64_t page;
@@ -38,59 +36,138 @@ __device__ inline Span span_of(const Cache& c, int b, int new_tokens, int nth) {
   return s;
 }
 
-template <Type TYPE>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs a) {
+// A thread's item: 4 slots of the page (one dword of a V row) by 8 dims (16 bytes of a 16-bit token).
+constexpr int kSlots = 4, kDims = 8;
+
+// KEEP: the items fit the threads, and a token is read once; else a second time for its codes.
+// VEC: every 8 elements of a token are a vector on a 16-byte boundary (fp32: two).
+template <Type TYPE, int THREADS, bool KEEP, bool VEC>
+__global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs a) {
   using T = typename Scalar<TYPE>::type;
-  __shared__ float lds[kThreads / 64];
+  __shared__ float lds[THREADS / 64];
   const Cache& c = a.cache;
   const int head = blockIdx.x, b = blockIdx.z >> 1, which = blockIdx.z & 1, tid = threadIdx.x;
   const Span s = span_of(c, b, a.new_tokens, blockIdx.y);
   if (s.n == 0) return;
+  const int page = 1 << c.page_shift, upto = s.slot0 + s.n;
   const T* x = static_cast<const T*>(a.x[which]) + b * a.stride_b[which] + head * a.stride_h[which];
   const int64_t st = a.stride_t[which];
+  uint8_t* pool = (which ? c.v : c.k) + (s.page * c.heads + head) * int64_t(page) * c.wide;
+  float* scale_at = (which ? c.v_scale : c.k_scale) + s.page * c.heads + head;
+  const float before = s.slot0 ? *scale_at : 0.0f;
+
+  const int octs = c.wide / kDims, quad0 = s.slot0 / kSlots, items = ((upto - 1) / kSlots - quad0 + 1) * octs;
+  float v[kSlots][kDims];
+  const auto load = [&](int item) {
+    const int slot = (quad0 + item / octs) * kSlots, d = item % octs * kDims;
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) {
+      const bool mine = slot + t >= s.slot0 && slot + t < upto;
+      const T* p = x + (s.first + slot + t - s.slot0) * st + d;
+      if (VEC) {
+        typedef T V __attribute__((ext_vector_type(kDims)));
+        const V r = mine && d < c.dim ? *reinterpret_cast<const V*>(p) : V{};
+#pragma unroll
+        for (int e = 0; e < kDims; ++e) v[t][e] = float(r[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kDims; ++e) v[t][e] = mine && d + e < c.dim ? float(p[e]) : 0.0f;
+      }
+    }
+  };
   // non-finite values do not set a scale: infinities are stored as the largest code, not-a-number as itself
   float amax = 0.0f;
-  for (int i = tid; i < s.n * c.dim; i += kThreads) {
-    const int t = i / c.dim, d = i - t * c.dim;
-    const float v = fabsf(float(x[(s.first + t) * st + d]));
-    amax = v < INFINITY ? fmaxf(amax, v) : amax;
+  for (int i = tid; i < items; i += THREADS) {
+    load(i);
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t)
+#pragma unroll
+      for (int e = 0; e < kDims; ++e) amax = fabsf(v[t][e]) < INFINITY ? fmaxf(amax, fabsf(v[t][e])) : amax;
   }
-  amax = block_reduce<kThreads>(amax, lds, Max());
-  float* scale_at = (which ? c.v_scale : c.k_scale) + s.page * c.heads + head;
-  const float fresh = pow2_scale(fmaxf(amax, kAmaxFloor)), before = s.slot0 ? *scale_at : 0.0f;
-  const float scale = fmaxf(fresh, before), inv = 1.0f / scale;
-  __syncthreads();
+  amax = block_reduce<THREADS>(amax, lds, Max());
+  const float scale = fmaxf(pow2_scale(fmaxf(amax, kAmaxFloor)), before), inv = 1.0f / scale;
+  if (THREADS > 64) __syncthreads();  // everybody has read the scale
   if (tid == 0) *scale_at = scale;
-  const int page = 1 << c.page_shift;
-  uint8_t* pool = (which ? c.v : c.k) + (s.page * c.heads + head) * int64_t(page) * c.wide;
-  const auto code = [&](float v) { return uint8_t(pack_fp8(v, 0.0f, 0.0f, 0.0f)); };
-  const auto clamped = [&](float v) { return v > kFp8Max ? kFp8Max : v < -kFp8Max ? -kFp8Max : v; };
-  const int upto = s.slot0 + s.n, old = scale > before ? 0 : s.slot0;  // slots that are written: [old, upto)
-  for (int i = tid; i < (upto - old) * c.wide; i += kThreads) {
-    const int row = i / c.wide, d = i - row * c.wide, slot = old + row;
-    uint8_t* p = pool + (which ? d * page + slot : slot * c.wide + d);
-    if (slot < s.slot0) {
-      const float v = __builtin_amdgcn_cvt_f32_fp8(int(*p), 0);
-      *p = code(v * (before * inv));
+
+  for (int i = tid; i < items; i += THREADS) {
+    if (!KEEP) load(i);
+    const int slot = (quad0 + i / octs) * kSlots, d = i % octs * kDims;
+    uint32_t code[kSlots][2];  // of a token's 8 dims
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) {
+#pragma unroll
+      for (int e = 0; e < kDims; ++e) {
+        const float w = v[t][e] * inv;
+        v[t][e] = w > kFp8Max ? kFp8Max : w < -kFp8Max ? -kFp8Max : w;
+      }
+      code[t][0] = pack_fp8(v[t][0], v[t][1], v[t][2], v[t][3]);
+      code[t][1] = pack_fp8(v[t][4], v[t][5], v[t][6], v[t][7]);
+    }
+    if (which == 0) {
+#pragma unroll
+      for (int t = 0; t < kSlots; ++t)
+        if (slot + t >= s.slot0 && slot + t < upto)
+          *reinterpret_cast<u32x2*>(pool + (slot + t) * c.wide + d) = u32x2{code[t][0], code[t][1]};
     } else {
-      const float v = d < c.dim ? float(x[(s.first + slot - s.slot0) * st + d]) : 0.0f;
-      *p = code(clamped(v * inv));
+      const bool all = slot >= s.slot0 && slot + kSlots <= upto;
+#pragma unroll
+      for (int e = 0; e < kDims; ++e) {
+        const uint32_t at = 8 * (e & 3);
+        uint32_t w = 0;
+#pragma unroll
+        for (int t = 0; t < kSlots; ++t) w |= (code[t][e >> 2] >> at & 0xff) << (8 * t);
+        uint8_t* p = pool + (d + e) * page + slot;
+        if (all) {
+          *reinterpret_cast<uint32_t*>(p) = w;
+        } else {
+#pragma unroll
+          for (int t = 0; t < kSlots; ++t)
+            if (slot + t >= s.slot0 && slot + t < upto) p[t] = uint8_t(w >> (8 * t));
+        }
+      }
     }
   }
+  if (scale > before) {  // the page's older tokens
+    for (int i = tid; i < s.slot0 * c.wide; i += THREADS) {
+      const int slot = i / c.wide, d = i - slot * c.wide;
+      uint8_t* p = pool + (which ? d * page + slot : i);
+      *p = uint8_t(pack_fp8(__builtin_amdgcn_cvt_f32_fp8(int(*p), 0) * (before * inv), 0.0f, 0.0f, 0.0f));
+    }
+  }
+}
+
+template <Type TYPE>
+void launch_type(const AppendArgs& a, Stream s) {
+  using T = typename Scalar<TYPE>::type;
+  const int page = 1 << a.cache.page_shift;
+  int64_t pages = (a.new_tokens - 1) / page + 2;
+  if (pages > a.cache.table_width) pages = a.cache.table_width;
+  const dim3 grid(a.cache.heads, unsigned(pages), 2 * a.batch);
+  bool vec = a.cache.dim % kDims == 0;
+  for (int w = 0; w < 2; ++w)
+    vec = vec && (reinterpret_cast<uintptr_t>(a.x[w]) | uintptr_t(a.stride_b[w] * sizeof(T)) |
+                  uintptr_t(a.stride_t[w] * sizeof(T)) | uintptr_t(a.stride_h[w] * sizeof(T))) % 16 == 0;
+  // the items of a page: a few tokens touch two quads at most for every four of them, and no more than the page has
+  const int quads = a.new_tokens < page ? (a.new_tokens + kSlots - 2) / kSlots + 1 : page / kSlots;
+  const int items = quads * (a.cache.wide / kDims);
+  const char* what = "kv_cache_append";
+  if (items <= 64)
+    launch(vec ? kv_append_kernel<TYPE, 64, true, true> : kv_append_kernel<TYPE, 64, true, false>, grid, 64, a, s, what);
+  else if (items <= 256)
+    launch(vec ? kv_append_kernel<TYPE, 256, true, true> : kv_append_kernel<TYPE, 256, true, false>, grid, 256, a, s,
+           what);
+  else
+    launch(vec ? kv_append_kernel<TYPE, 256, false, true> : kv_append_kernel<TYPE, 256, false, false>, grid, 256, a, s,
+           what);
 }
 
 }  // namespace
 
 void kv_append_hip(const AppendArgs& a, Stream s) {
-  if (a.batch == 0 || a.new_tokens == 0 || a.cache.heads == 0 || a.cache.table_width == 0) return;
-  const int page = 1 << a.cache.page_shift;
-  int64_t pages = (a.new_tokens - 1) / page + 2;
-  if (pages > a.cache.table_width) pages = a.cache.table_width;
-  const dim3 grid(a.cache.heads, unsigned(pages), 2 * a.batch);
-  const auto k = a.type == kF32   ? kv_append_kernel<kF32>
-                 : a.type == kF16 ? kv_append_kernel<kF16>
-                                  : kv_append_kernel<kBF16>;
-  launch(k, grid, kThreads, a, s, "kv_cache_append");
+  if (a.batch == 0 || a.new_tokens == 0 || a.cache.table_width == 0) return;
+  if (a.type == kF32) return launch_type<kF32>(a, s);
+  if (a.type == kF16) return launch_type<kF16>(a, s);
+  launch_type<kBF16>(a, s);
 }
 
 }  // namespace tl_ops

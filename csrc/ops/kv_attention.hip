@@ -126,9 +126,10 @@ __device__ inline void poison(bf16x8 is, bool there, int key, int pos, f32x4& o)
 }
 
 // The weights of 16 scores of each of NR rows (in units of 1 / ks), with V's scale, as operands of the second
-// product; a page that is not `there` has none.  The sums are relative to m, which moves only when the scores outgrow it by more than 2^8: weights up to
-// 2^8 lose nothing in bf16 and float32.
-template <Type TYPE, int NR, int DT>
+// product; a page that is not `there` has none.  The sums are relative to m, which moves when the scores outgrow it by
+// more than a factor of 2^SLACK.  With 0 the largest weight is 1 and rounds to itself; a larger one saves most of the
+// sums' rescaling where that counts (weights up to 2^SLACK fit bf16 and float32 as well).
+template <Type TYPE, int NR, int DT, int SLACK>
 __device__ inline void softmax_step(const f32x4 (&s)[NR][4], float ks, float vs, bool there, float (&m)[NR],
                                     float (&l)[NR], f32x4 (&o)[NR][DT], bf16x8 (&hi)[NR][2], bf16x8 (&lo)[NR][2]) {
   float top[NR];
@@ -141,7 +142,7 @@ __device__ inline void softmax_step(const f32x4 (&s)[NR][4], float ks, float vs,
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[r] = fmaxf(top[r], s[r][t][i]);
     top[r] = across_groups(there ? top[r] * ks : -INFINITY, Max());
-    grown |= top[r] > m[r] + 8.0f;
+    grown |= top[r] > m[r] + float(SLACK);
   }
   if (__any(grown)) {
 #pragma unroll
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
     const float ks = fmaxf(now.ks * to_log2, 1e-30f);  // never zero: a hidden score stays -inf
     const float vs = now.there ? now.vs : 0.0f;
     bf16x8 hi[NR][2], lo[NR][2];
-    softmax_step<TYPE, NR, DT>(s, ks, vs, now.there, m, l, o, hi, lo);
+    softmax_step<TYPE, NR, DT, 0>(s, ks, vs, now.there, m, l, o, hi, lo);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv_attention_chunk_kernel(At
       for (int r = 0; r < NR; ++r) hide(s[r], now.there, key_v, pos[r]);
     }
     bf16x8 hi[NR][2], lo[NR][2];
-    softmax_step<TYPE, NR, DT>(s, fmaxf(now.ks * to_log2, 1e-30f), now.vs, now.there, m, l, o, hi, lo);
+    softmax_step<TYPE, NR, DT, 8>(s, fmaxf(now.ks * to_log2, 1e-30f), now.vs, now.there, m, l, o, hi, lo);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll

@@ -100,16 +100,18 @@ struct BeamArgs {
   int beams, take, vocab;
   Type type;
   int chunks;           // parts of the vocabulary: beam_select_chunks()
-  float* part_stat;     // [batch * beams, chunks, 2]
+  float* part_stat;     // [batch * beams, chunks, waves, 2]
   uint64_t* part_list;  // [batch * beams, chunks, take]
 };
 
 constexpr int kBeamMaxTake = 64;
 constexpr int kBeamMaxBeams = 64;
+constexpr int kBeamMaxVocab = 1 << 20;
 constexpr int kBeamMaxLists = 4096;  // beams * chunks
 
-int beam_select_chunks(int64_t rows, int vocab);
-void beam_select_hip(const BeamArgs&, Stream);
+int beam_select_chunks(int vocab);
+int64_t beam_select_scratch(int64_t rows, int chunks, int take);  // 8-byte words of scratch memory
+void beam_select_hip(BeamArgs, uint64_t* scratch, Stream);
 void beam_select_cpu(const BeamArgs&);
 
 struct ReorderState {

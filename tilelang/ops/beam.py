@@ -16,8 +16,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: Optional[int] 
                 eos_id: int = -1) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``take`` best continuations of every sequence's beams (default: as many as beams, at most 64).
 
-    logits [batch, beams, vocab] or [batch * beams, vocab] (fp32, bf16, fp16), scores float32 [batch, beams] (the
-    beams' sums of log probabilities; -inf for a beam that is not in use).  The value of token t after beam k is
+    logits [batch, beams, vocab] or [batch * beams, vocab] (fp32, bf16, fp16; at most 64 beams and 2^20 tokens),
+    scores float32 [batch, beams] (the beams' sums of log probabilities; -inf for a beam that is not in use).  The
+    value of token t after beam k is
 
         scores[k] + logits[k, t] - logsumexp(logits[k])
 
