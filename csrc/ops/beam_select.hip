@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKept = 512;        // candidates of a chunk that LDS takes
 constexpr int kMergeKept = 2048;  // and of a sequence
 
@@ -73,8 +74,19 @@ __device__ inline int slot_for(bool keep, int* count) {
   return base + int(__builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0)));
 }
 
+// The place of a candidate among n: eight lanes count the larger ones together.
+template <typename C, typename F>
+__device__ inline int place_of(const C* kept, int n, const C& mine, F before) {
+  int place = 0;
+  for (int j = threadIdx.x & 7; j < n; j += 8) place += before(kept[j], mine);
+#pragma unroll
+  for (int m = 1; m < 8; m <<= 1) place += __shfl_xor(place, m);
+  return place;
+}
+
+// (eight waves to a SIMD: 2048 chunks, 8 rows of 129280 tokens for each of 8 beams, are in flight at once)
 template <Type TYPE, int PER>
-__global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamArgs a) {
+__global__ __launch_bounds__(kThreads, PER == 16 ? 8 : 1) void beam_scan_kernel(BeamArgs a) {
   using T = typename Scalar<TYPE>::type;
   constexpr int VEC = 16 / sizeof(T), VECS = PER / VEC, CHUNK = kThreads * PER;
   __shared__ uint32_t t_lds[kWaves];
@@ -115,9 +127,10 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamArgs a) {
   if ((tid & 63) == 0) t_lds[wave] = t;
   top = wave_reduce(top, Max());
   float sum = 0.0f;
+  if (top > -INFINITY) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    sum += top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v[j] - top) * 1.4426950408889634f);
+    for (int j = 0; j < PER; ++j) sum += __builtin_amdgcn_exp2f((v[j] - top) * kLog2e);
+  }
   sum = wave_reduce(nan ? NAN : sum, Add());
   const int64_t list = row * a.chunks + chunk;
   if ((tid & 63) == 0) {
@@ -126,9 +139,10 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamArgs a) {
     stat[1] = sum;
   }
   __syncthreads();
-  uint32_t limit = 1;
+  uint32_t limit = order_of(-INFINITY);
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) limit = t_lds[w] > limit ? t_lds[w] : limit;
+  const float least = from_order(limit);
 
   const auto key_of = [&](int j) -> uint64_t {
     const int token = at(j / VEC, j % VEC);
@@ -136,22 +150,20 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamArgs a) {
   };
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const uint64_t key = key_of(j);
-    const bool keep = uint32_t(key >> 32) >= limit;
+    const bool keep = v[j] >= least && at(j / VEC, j % VEC) < left;
     if (__any(keep)) {
       const int s = slot_for(keep, &count);
-      if (keep && s < kKept) kept[s] = key;
+      if (keep && s < kKept) kept[s] = key_of(j);
     }
   }
   __syncthreads();
   const int n = count;
   uint64_t* out = a.part_list + list * a.take;
   if (n <= kKept) {
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid >> 3; i < n; i += kThreads / 8) {
       const uint64_t key = kept[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += kept[j] > key;
-      if (place < a.take) out[place] = key;
+      const int place = place_of(kept, n, key, [](uint64_t x, uint64_t y) { return x > y; });
+      if ((tid & 7) == 0 && place < a.take) out[place] = key;
     }
     for (int i = n + tid; i < a.take; i += kThreads) out[i] = 0;  // the chunk has no more
     return;
@@ -180,16 +192,25 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamArgs a) {
   }
 }
 
+constexpr int kNone = INT32_MAX;
+
 struct Candidate {
   double value;
-  int64_t at;  // beam * vocab + token; INT64_MAX: none
+  int at;  // beam * vocab + token, less than 2^26; kNone: no candidate
 };
 __device__ inline bool before(const Candidate& a, const Candidate& b) {
   return a.value > b.value || (a.value == b.value && a.at < b.at);
 }
-__device__ inline Candidate shuffle(const Candidate& c, int m) {
-  return {__shfl_xor(c.value, m), (int64_t)__shfl_xor((long long)c.at, m)};
-}
+__device__ inline Candidate shuffle(const Candidate& c, int m) { return {__shfl_xor(c.value, m), __shfl_xor(c.at, m)}; }
+
+// A beam's chunk: its candidates are in order.  A beam without a finite score or logsumexp has only -inf to offer, a
+// finished one its eos token and -inf: their tokens are counted off by the beam's first list.
+struct List {
+  const uint64_t* keys;  // null: there is no such list
+  int beam, chunk;
+  float score;
+  bool done;
+};
 
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   __shared__ double lse_lds[kBeamMaxBeams];
@@ -199,52 +220,66 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   __shared__ int count;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
-  const double inf = INFINITY;
   if (tid == 0) count = 0;
+
+  // The first keys of the thread's first list are on their way while the statistics are joined.
+  const int lists = a.beams * a.chunks;
+  const auto list_of = [&](int j) -> List {
+    if (j >= lists) return {nullptr, 0, 0, 0.0f, false};
+    const int k = j / a.chunks;
+    const int64_t row = b * a.beams + k;
+    return {a.part_list + (row * a.chunks + (j - k * a.chunks)) * a.take, k, j - k * a.chunks, a.scores[row],
+            a.finished && a.finished[row]};
+  };
+  const auto key_of = [&](const List& l, int nth) { return l.keys && nth < a.take ? l.keys[nth] : 0; };
+  const int lanes = lists < 64 ? lists : 64, nth = (a.take - 1) / lanes, q = (a.take + nth) / (nth + 1);
+  constexpr int kAhead = 4;
+  const List own = list_of(tid);
+  uint64_t own_keys[kAhead];
+#pragma unroll
+  for (int e = 0; e < kAhead; ++e) own_keys[e] = key_of(own, e);
+  const uint64_t own_nth = key_of(own, nth);
+
+  constexpr int kStats = 64 * kWaves / 64;  // a row has at most 64 chunks
   for (int k = wave; k < a.beams; k += kMergeWaves) {
     const int n = a.chunks * kWaves;
     const float* stat = a.part_stat + (b * a.beams + k) * n * 2;
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, stat[2 * i]);
+    float m[kStats], l[kStats], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kStats; ++i) {
+      const bool mine = 64 * i + lane < n;
+      m[i] = mine ? stat[2 * (64 * i + lane)] : -INFINITY;
+      l[i] = mine ? stat[2 * (64 * i + lane) + 1] : 0.0f;
+      top = fmaxf(top, m[i]);
+    }
     top = wave_reduce(top, Max());
     double sum = 0.0;  // not-a-number where a wave's is, or where the maximum is infinite: such a beam is dead
-    for (int i = lane; i < n; i += 64)
-      sum += double(stat[2 * i + 1]) * double(__builtin_amdgcn_exp2f((stat[2 * i] - top) * 1.4426950408889634f));
+#pragma unroll
+    for (int i = 0; i < kStats; ++i) sum += double(l[i]) * double(__builtin_amdgcn_exp2f((m[i] - top) * kLog2e));
     sum = wave_sum(sum);
     if (lane == 0) lse_lds[k] = double(top) + log(sum);
   }
   __syncthreads();
 
-  // List j belongs to beam j / chunks.  A beam without a finite score or logsumexp has only -inf to offer, a
-  // finished one its eos token and -inf: their tokens are counted off by the beam's first list.
-  const int lists = a.beams * a.chunks;
-  const auto candidate = [&](int j, int nth) -> Candidate {
-    const int k = j / a.chunks, c = j - k * a.chunks;
-    const int64_t none = INT64_MAX, first = int64_t(k) * a.vocab;
-    if (j >= lists || nth >= a.take) return {-inf, none};
-    const float score = a.scores[b * a.beams + k];
-    const double lse = lse_lds[k];
-    const bool live = fabsf(score) < INFINITY, done = a.finished && a.finished[b * a.beams + k];
-    if (done && live) {
-      if (c || nth >= a.vocab) return {-inf, none};
-      if (nth == 0) return {double(score), first + a.eos};
-      return {-inf, first + (nth - 1 < a.eos ? nth - 1 : nth)};
+  const auto candidate = [&](const List& l, uint64_t key, int nth) -> Candidate {
+    const double none = -INFINITY;
+    const int first = l.beam * a.vocab;
+    if (!l.keys || nth >= a.take) return {none, kNone};
+    const double lse = lse_lds[l.beam];
+    const bool finite = fabsf(l.score) < INFINITY, done = l.done && finite;
+    if (done || !finite || !(fabs(lse) < double(INFINITY))) {
+      if (l.chunk || nth >= a.vocab) return {none, kNone};
+      if (done && nth == 0) return {double(l.score), first + int(a.eos)};
+      return {none, first + (done && nth - 1 < a.eos ? nth - 1 : nth)};
     }
-    if (!live || !(fabs(lse) < inf)) {
-      if (c || nth >= a.vocab) return {-inf, none};
-      return {-inf, first + nth};
-    }
-    const uint64_t key = a.part_list[((b * a.beams + k) * a.chunks + c) * a.take + nth];
-    if (key == 0) return {-inf, none};
-    const double x = from_order(uint32_t(key >> 32));
-    return {double(score) + (x - lse), first + uint32_t(~uint32_t(key))};
+    if (key == 0) return {none, kNone};
+    return {double(l.score) + (double(from_order(uint32_t(key >> 32))) - lse), first + int(~uint32_t(key))};
   };
-  const auto order = [&](const Candidate& c) { return c.at == INT64_MAX ? 0u : order_of(c.value); };
+  const auto order = [&](const Candidate& c) { return c.at == kNone ? 0u : order_of(c.value); };
 
-  // If q lists' candidates number j (from 0) reach T, the best q (j + 1) do: T is such that this is `take`.
-  const int lanes = lists < 64 ? lists : 64, nth = (a.take - 1) / lanes, q = (a.take + nth) / (nth + 1);
+  // If q lists' candidates number `nth` (from 0) reach T, the best q (nth + 1) do: T is such that this is `take`.
   if (wave * 64 < lists) {
-    const uint32_t t = reached_by<0>(order(candidate(tid, nth)), q);
+    const uint32_t t = reached_by<8>(order(candidate(own, own_nth, nth)), q);
     if (lane == 0) t_lds[wave] = t;
   } else if (lane == 0) {
     t_lds[wave] = 0;
@@ -253,16 +288,22 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   uint32_t limit = 1;
 #pragma unroll
   for (int w = 0; w < kMergeWaves; ++w) limit = t_lds[w] > limit ? t_lds[w] : limit;
-  // lists are in order: each is read up to its first candidate below T
+  // Lists are in order: each is read up to its first candidate below T
   for (int j0 = 0; j0 < lists; j0 += kMergeThreads) {
-    bool open = j0 + tid < lists;
-    for (int i = 0; i < a.take; ++i) {
-      Candidate c{-inf, INT64_MAX};
-      if (open) c = candidate(j0 + tid, i);
-      open = open && order(c) >= limit;
-      if (!__any(open)) break;
-      const int s = slot_for(open, &count);
-      if (open && s < kMergeKept) kept[s] = c;
+    const List l = j0 ? list_of(j0 + tid) : own;
+    bool open = true;
+    for (int i = 0; i < a.take && __any(open); i += kAhead) {
+      uint64_t key[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) key[e] = j0 + i ? key_of(l, i + e) : own_keys[e];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const Candidate c = candidate(l, key[e], i + e);
+        open = open && order(c) >= limit;
+        if (!__any(open)) break;
+        const int s = slot_for(open, &count);
+        if (open && s < kMergeKept) kept[s] = c;
+      }
     }
   }
   __syncthreads();
@@ -273,11 +314,10 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   };
   const int n = count;
   if (n <= kMergeKept) {
-    for (int i = tid; i < n; i += kMergeThreads) {
+    for (int i = tid >> 3; i < n; i += kMergeThreads / 8) {
       const Candidate c = kept[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) place += before(kept[j], c);
-      if (place < a.take) write(place, c);
+      const int place = place_of(kept, n, c, before);
+      if ((tid & 7) == 0 && place < a.take) write(place, c);
     }
     return;
   }
@@ -286,14 +326,15 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   uint8_t taken[kOwn];
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) taken[i] = 0;
-  Candidate mine{-inf, INT64_MAX};
+  Candidate mine{-double(INFINITY), kNone};
   int mine_list = -1;
   const auto look = [&] {
-    mine = {-inf, INT64_MAX};
+    mine = {-double(INFINITY), kNone};
     mine_list = -1;
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const Candidate h = candidate(i * kMergeThreads + tid, taken[i]);
+      const List l = list_of(i * kMergeThreads + tid);
+      const Candidate h = candidate(l, key_of(l, taken[i]), taken[i]);
       if (before(h, mine)) mine = h, mine_list = i;
     }
   };
