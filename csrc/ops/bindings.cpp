@@ -60,8 +60,8 @@ struct Call {
     NEED(t.size(d) == n, name, ": argument '", arg, "' dim ", d, " is ", t.size(d), ", expected ", n);
   }
   void dtype(const Tensor& t, const char* arg, c10::ScalarType s) const {
-    NEED_AS(py::type_error, t.scalar_type() == s, name, ": argument '", arg, "' has dtype ", c10::toString(t.scalar_type()),
-              ", expected ", c10::toString(s));
+    NEED_AS(py::type_error, t.scalar_type() == s, name, ": argument '", arg, "' has dtype ",
+            c10::toString(t.scalar_type()), ", expected ", c10::toString(s));
   }
   void contiguous(const Tensor& t, const char* arg) const {
     NEED(t.is_contiguous(), name, ": argument '", arg, "' must be contiguous");
@@ -375,7 +375,7 @@ void reorder_states(const std::vector<Tensor>& states, const Tensor& parents, co
     const int64_t bytes = moves * int64_t(t.element_size()), stride = t.stride(0) * int64_t(t.element_size());
     if (bytes == 0) continue;
     NEED(rows == 1 || stride >= bytes, c.name, ": a state's rows overlap");
-    moved.push_back({static_cast<uint8_t*>(t.data_ptr()), stride, bytes});
+    moved.push_back({static_cast<uint8_t*>(t.data_ptr()), stride, bytes, 0});
   }
   // No byte may be moved twice.  In the order of their addresses, two states that share a range must be columns of
   // one buffer: rows equally far apart, the second's bytes behind the first's and before its next row.

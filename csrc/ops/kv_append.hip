@@ -152,7 +152,8 @@ void launch_type(const AppendArgs& a, Stream s) {
   const int items = quads * (a.cache.wide / kDims);
   const char* what = "kv_cache_append";
   if (items <= 64)
-    launch(vec ? kv_append_kernel<TYPE, 64, true, true> : kv_append_kernel<TYPE, 64, true, false>, grid, 64, a, s, what);
+    launch(vec ? kv_append_kernel<TYPE, 64, true, true> : kv_append_kernel<TYPE, 64, true, false>, grid, 64, a, s,
+           what);
   else if (items <= 256)
     launch(vec ? kv_append_kernel<TYPE, 256, true, true> : kv_append_kernel<TYPE, 256, true, false>, grid, 256, a, s,
            what);

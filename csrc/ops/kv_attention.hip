@@ -18,6 +18,7 @@
 //
 // The waves of a workgroup take tiles in turn and join in LDS; `splits` workgroups share a long key axis and
 // kv_join_kernel joins them.
+#include <algorithm>
 #include <type_traits>
 
 #include "device.h"
@@ -187,6 +188,14 @@ __device__ inline void store4(T* row, f32x4 v, int at, int dim) {
   }
 }
 
+// STREAM: past the caches.  For what they could not keep until it is read again: 32 sequences of 4096 to 8192 tokens
+// (400 MB) take 74.7 us with it and 80.9 without, 16 of 1024 to 2048 in heads of 100 (206 MB) 40.3 and 34.6.
+template <bool STREAM>
+__device__ inline u32x4 load16(const uint8_t* p) {
+  const u32x4* q = reinterpret_cast<const u32x4*>(p);
+  return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+
 // The pages of a lane's K row and of its 16 keys in one tile, and where they are.  Pages of 64 tokens and more hold
 // WHOLE tiles: then both are one page for all lanes, and its id, address and scales stay in scalar registers.
 struct Pages {
@@ -198,7 +207,7 @@ struct Place {
   bool there;  // whether the page of its 16 keys is in the pool
 };
 
-template <Type TYPE, int DC, int NR, bool WHOLE>
+template <Type TYPE, int DC, int NR, bool WHOLE, bool STREAM>
 __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a) {
   using T = typename Scalar<TYPE>::type;
   constexpr int ROWS = 16 * NR, DT = 4 * DC;  // rows of the workgroup, 16-wide slices of the head
@@ -251,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int k = 0; k < DC; ++k) kx[t][k] = *reinterpret_cast<const u32x4*>(p.k + 4 * t * c.wide + 64 * k);
+      for (int k = 0; k < DC; ++k) kx[t][k] = load16<STREAM>(p.k + 4 * t * c.wide + 64 * k);
   };
   // What a tile needs is asked for a tile ahead (its pages' ids two ahead), and V behind K: no wait is for a load
   // that has just been issued.  Behind the last tile the loads repeat it.
@@ -284,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
     const Place now = at;
 #pragma unroll
     for (int d = 0; d < DT; ++d)  // a padded row is not read: another one stands in, its result is not written
-      vx[d] = *reinterpret_cast<const u32x4*>(now.v + (16 * d + col < c.dim ? 16 * d + col : c.dim - 1) * page);
+      vx[d] = load16<STREAM>(now.v + (16 * d + col < c.dim ? 16 * d + col : c.dim - 1) * page);
     at = place_of(ahead(tile + kWaves), next);
     next = pages_of(ahead(tile + 2 * kWaves));
 
@@ -690,12 +699,18 @@ void launch_dim(const AttentionArgs& a, Stream s) {
   const dim3 grid(unsigned(a.cache.heads * ceil_div(rows, tile)), a.splits, a.batch);
   const bool whole = 1 << a.cache.page_shift >= kTile;
   const char* what = "kv_cache_attention";
-  if (tile == 16)
-    launch(whole ? kv_attention_kernel<TYPE, DC, 1, true> : kv_attention_kernel<TYPE, DC, 1, false>, grid, kThreads, a,
-           s, what);
+  // what one call reads of the cache at most, against the 256 MB of the last cache
+  const int64_t pages = std::min(int64_t(a.batch) * a.cache.table_width, a.cache.pages);
+  const bool stream = (pages * a.cache.heads * a.cache.wide << (a.cache.page_shift + 1)) > (int64_t(256) << 20);
+  if (tile == 16 && stream)
+    launch(whole ? kv_attention_kernel<TYPE, DC, 1, true, true> : kv_attention_kernel<TYPE, DC, 1, false, true>, grid,
+           kThreads, a, s, what);
+  else if (tile == 16)
+    launch(whole ? kv_attention_kernel<TYPE, DC, 1, true, false> : kv_attention_kernel<TYPE, DC, 1, false, false>,
+           grid, kThreads, a, s, what);
   else if (tile == 32)
-    launch(whole ? kv_attention_kernel<TYPE, DC, 2, true> : kv_attention_kernel<TYPE, DC, 2, false>, grid, kThreads, a,
-           s, what);
+    launch(whole ? kv_attention_kernel<TYPE, DC, 2, true, false> : kv_attention_kernel<TYPE, DC, 2, false, false>,
+           grid, kThreads, a, s, what);
   else if constexpr (DC <= 2)
     launch(whole ? kv_attention_chunk_kernel<TYPE, DC, true> : kv_attention_chunk_kernel<TYPE, DC, false>, grid,
            kChunkThreads, a, s, what);

@@ -6,6 +6,8 @@
 // the codes come from the unrounded y.  One workgroup owns a row and keeps it in registers (NV vectors of 8
 // elements per thread), so every input byte is read once.  A vector belongs to one scale group; the lanes that
 // hold a group are neighbours and reduce its maximum among themselves.
+//
+// Bound by HBM: 7 bytes an element with a residual in 16 bits.  8192 x 7168 bf16: 79 us, 5.2 TB/s.
 #include "device.h"
 
 namespace tl_ops {
@@ -138,11 +140,13 @@ void launch_type(const NormQuantArgs& a, Stream s) {
   const auto on16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool whole = a.width % 8 == 0 && on16(a.x) && on16(a.residual) && on16(a.weight) &&
                      a.x_stride * bytes % 16 == 0 && a.residual_stride * bytes % 16 == 0;
+  // Few vectors to a thread keep rows in flight; 7168 wide, 8192 rows: 512 threads by 2 79.2 us, 256 by 4 85.6, 1024
+  // by 1 85.1; 64 rows: 5.7, 6.8, 6.0.
   const int vectors = int(ceil_div(a.width, 8));
   if (vectors <= 64) return launch_rows<TYPE, 64, 1>(a, whole, s);
   if (vectors <= 256) return launch_rows<TYPE, 256, 1>(a, whole, s);
   if (vectors <= 512) return launch_rows<TYPE, 256, 2>(a, whole, s);
-  if (vectors <= 1024) return launch_rows<TYPE, 256, 4>(a, whole, s);
+  if (vectors <= 1024) return launch_rows<TYPE, 512, 2>(a, whole, s);
   if (vectors <= 2048) return launch_rows<TYPE, 512, 4>(a, whole, s);
   launch_rows<TYPE, 1024, 8>(a, whole, s);
 }

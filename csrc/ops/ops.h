@@ -118,6 +118,7 @@ struct ReorderState {
   uint8_t* data;
   int64_t stride;  // bytes between two rows
   int64_t bytes;   // bytes of a row that move
+  int64_t first;   // the first of its workgroups
 };
 
 constexpr int kReorderMaxBeams = 32;
@@ -130,7 +131,7 @@ struct ReorderArgs {
   int beams, states;
 };
 
-void reorder_hip(const ReorderArgs&, Stream);
+void reorder_hip(ReorderArgs, Stream);
 void reorder_cpu(const ReorderArgs&);
 
 }  // namespace tl_ops
