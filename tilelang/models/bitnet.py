@@ -15,7 +15,8 @@ MI355X execution (``tilelang.ops.bitnet``):
   2 bits each in HBM, per-column weight scales in the dequantising epilogue); decode-sized inputs
   (<= 8 rows) take the weight-streaming GEMV kernel instead (no matrix cores, K padded to 256);
 * attention uses PyTorch SDPA (the BitNet-specific work is the ternary projections; the flash
-  kernels live in examples/flash_attention).
+  kernels live in examples/flash_attention); ``generate_cached`` decodes from an e4m3 paged key/value cache
+  (``tilelang.ops.kv_cache``) instead of recomputing the sequence, greedily or with beams (``tilelang.ops.beam``).
 
 Weights are random (no checkpoint is available offline); ``BitnetConfig.bitnet_3b()`` is the
 reference's 3B shape.  ``reference_forward`` is the reference's fp32-simulated BitLinear math,
@@ -31,6 +32,8 @@ import torch
 from torch import nn
 
 from ..ops import bitnet as K
+from ..ops.beam import beam_select, reorder_states
+from ..ops.kv_cache import alloc_kv_cache, kv_cache_append, kv_cache_attention
 
 
 @dataclass
@@ -119,7 +122,8 @@ class BitnetDecoderLayer(nn.Module):
         self.gate_up = BitLinearGroup(h, [i, i], dt)
         self.down = BitLinearGroup(i, [h], dt)
 
-    def forward(self, x, cos, sin):
+    def forward(self, x, cos, sin, attend=None):
+        """``attend(q, k, v)`` [b, s, heads, head_dim] replaces the attention among the given tokens."""
         cfg = self.cfg
         b, s, h = x.shape
         nh = cfg.num_attention_heads
@@ -129,8 +133,11 @@ class BitnetDecoderLayer(nn.Module):
         q, k, v = self.qkv(xq, sx, x.dtype)
         q, k, v = (t.view(b, s, nh, hd).transpose(1, 2) for t in (q, k, v))
         q, k = _rope(q, cos, sin), _rope(k, cos, sin)
-        a = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True)
-        a = a.transpose(1, 2).reshape(b, s, h)
+        if attend is None:
+            a = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2)
+        else:
+            a = attend(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+        a = a.reshape(b, s, h)
         aq, sa = K.rms_norm_quant(a, self.inner_attn_ln, eps)
         x = x + self.o_proj(aq, sa, x.dtype)
         xq, sx = K.rms_norm_quant(x, self.post_attention_layernorm, eps)
@@ -170,6 +177,66 @@ class BitnetForCausalLM(nn.Module):
             nxt = self.forward(ids)[:, -1].argmax(-1, keepdim=True)
             ids = torch.cat([ids, nxt], 1)
         return ids
+
+
+    @torch.no_grad()
+    def _step(self, ids, start: int, caches, table, lengths):
+        """Logits of the last of the tokens ``ids``, which take the positions from ``start``."""
+        from ..ops.norm import rms_norm
+        cfg = self.cfg
+        x = self.embed_tokens[ids]
+        s = ids.shape[1]
+        cos, sin = rope_tables(cfg.hidden_size // cfg.num_attention_heads, start + s, cfg.rope_theta, x.device, x.dtype)
+        for layer, cache in zip(self.layers, caches):
+
+            def attend(q, k, v, cache=cache):
+                kv_cache_append(cache, k, v, table, lengths)
+                return kv_cache_attention(q, cache, table, lengths)
+
+            x = layer(x, cos[start:], sin[start:], attend)
+        return rms_norm(x[:, -1], self.norm, cfg.rms_norm_eps) @ self.lm_head.t()
+
+    @torch.no_grad()
+    def generate_cached(self, input_ids: torch.Tensor, max_new_tokens: int = 8, beams: int = 1, eos_id: int = -1,
+                        page_size: int = 64):
+        """Decoding from an e4m3 key/value cache: one forward of the prompt, then one of a token per step.
+
+        ``beams`` = 1: greedy, [b, s + max_new_tokens] as ``generate``.  More: beam search, (ids [b, beams, s +
+        max_new_tokens], scores [b, beams]), best first; a beam that has ended repeats ``eos_id``."""
+        cfg, dev = self.cfg, input_ids.device
+        b, start = input_ids.shape
+        if not 1 <= beams <= 32:
+            raise ValueError(f"generate_cached: {beams} beams, expected 1 to 32")
+        total = start + max_new_tokens
+        rows, pages, heads = b * beams, -(-total // page_size), cfg.num_attention_heads
+        caches = [alloc_kv_cache(rows * pages, heads, cfg.hidden_size // heads, page_size, dev) for _ in self.layers]
+        # every row has its own pages, so that the pools are states [rows, pages of a row, ...]
+        table = torch.arange(rows * pages, dtype=torch.int32, device=dev).view(rows, pages)
+        states = [t.view(rows, pages, -1) for c in caches for t in c[:4]]
+        ids = torch.zeros(rows, total, dtype=torch.long, device=dev)
+        ids[:, :start] = input_ids.repeat_interleave(beams, 0)
+        scores = torch.full((b, beams), float("-inf"), device=dev)
+        scores[:, 0] = 0.0  # the beams of a prompt are still one
+        finished = torch.zeros(b, beams, dtype=torch.bool, device=dev) if eos_id >= 0 else None
+        # the prompt goes through once, into the first beam's pages, which are then every beam's
+        lengths = torch.full((rows, ), start, dtype=torch.int32, device=dev)
+        logits = self._step(input_ids, 0, caches, table[::beams], lengths[::beams].contiguous())
+        logits = logits.repeat_interleave(beams, 0)
+        reorder_states(states, torch.zeros(b, beams, dtype=torch.long, device=dev), -(-start // page_size))
+        for cur in range(start, total):
+            if beams == 1:
+                ids[:, cur] = logits.argmax(-1)
+            else:
+                scores, parents, nxt = beam_select(logits, scores, finished=finished, eos_id=eos_id)
+                reorder_states(states, parents, -(-cur // page_size))
+                reorder_states([ids], parents, cur)
+                ids[:, cur] = nxt.flatten()
+                if finished is not None:
+                    finished = finished.gather(1, parents) | (nxt == eos_id)
+            if cur + 1 < total:
+                lengths += 1
+                logits = self._step(ids[:, cur:cur + 1], cur, caches, table, lengths)
+        return ids if beams == 1 else (ids.view(b, beams, total), scores)
 
 
 # ---------------------------------------------------------------------------------------- fp32 oracle

@@ -21,12 +21,15 @@ RCCL over xGMI); every projection is a tilelang MFMA GEMM; fp8 is OCP e4m3 (gfx9
 in the checkpoint's fp8 format -- OCP e4m3 with one fp32 scale per 128x128 block -- and runs it
 as ``act_quant`` (per-token, 128-wide groups; ``scale_fmt="ue8m0"`` for power-of-two scales) +
 the block-scaled fp8 GEMM (``tilelang.ops.fp8_gemm``, 2xAcc promotion), as the reference's
-``linear`` does (model.py:140-168).  The absorbed MLA up-projection dequantises ``wkv_b`` once
-(``weight_dequant``, model.py:514, cached as model.py:625 does) and runs as per-head MFMA GEMMs
+``linear`` does (model.py:140-168).  ``ModelArgs.norm_quant = "fused"`` writes that operand in the norm itself
+(``ops.norm.add_rms_norm_quant``: residual addition, norm and fp8 cast in one pass, shared by every projection
+that reads the row; the codes then come from the unrounded norm).  The absorbed MLA up-projection dequantises
+``wkv_b`` once (``weight_dequant``, model.py:514, cached as model.py:625 does) and runs as per-head MFMA GEMMs
 (``tilelang.ops.gemm.head_bmm``); routed experts stay on the bf16 grouped-GEMM kernels.
 Checkpoints: ``tilelang.models.deepseek_v32_ckpt`` converts HF-named safetensors into per-rank
 ``model{rank}-mp{world}.safetensors`` shards and loads them (reference convert.py /
-generate.py:119).
+generate.py:119).  ``generate`` is greedy / sampled, ``generate_beams`` a beam search whose selection and cache
+reordering stay on the device (``ops.beam``).
 
 Simplifications (documented; no real checkpoint is available offline, so tests round-trip
 synthetic weights through convert -> load): plain RoPE (no YaRN rescaling), no Hadamard rotation
@@ -42,9 +45,10 @@ import torch.distributed as dist
 from torch import nn
 
 from ..ops import dsa
+from ..ops.beam import beam_select, reorder_states
 from ..ops.gemm import head_bmm, linear
 from ..ops.moe import expert_ffn
-from ..ops.norm import rms_norm
+from ..ops.norm import NormQuant, add_rms_norm_quant, rms_norm
 from ..ops.quant import act_quant
 
 
@@ -80,6 +84,7 @@ class ModelArgs:
     block_M: int = 128  # MoE row tile
     gemm_impl: str = "bf16"  # "fp8": block-scaled fp8 projection weights (the checkpoint format)
     scale_fmt: Optional[str] = None  # "ue8m0": power-of-two activation scales
+    norm_quant: str = "separate"  # "fused": the norms in front of fp8 projections write their operand
 
     @staticmethod
     def from_json(path: str, **over) -> "ModelArgs":
@@ -155,10 +160,13 @@ class Linear(nn.Module):
         else:
             self.weight = nn.Parameter(w.contiguous(), requires_grad=False)
 
-    def _mm(self, x):
+    def _mm(self, x, xq: Optional[NormQuant] = None):
+        """``xq``: x as a fused norm quantised it, for fp8 weights."""
         if self.scale is None:
             return linear(x, self.weight)
-        from ..ops.fp8_gemm import fp8_linear
+        from ..ops.fp8_gemm import fp8_gemm, fp8_linear
+        if xq is not None:
+            return fp8_gemm(xq.q, xq.scale, self.weight, self.scale, self.out_dtype)
         return fp8_linear(x.to(self.out_dtype), self.weight, self.scale, Linear.scale_fmt == "ue8m0")
 
     def dequant_weight(self) -> torch.Tensor:
@@ -168,8 +176,8 @@ class Linear(nn.Module):
         from ..ops.fp8_gemm import weight_dequant
         return weight_dequant(self.weight, self.scale).to(self.out_dtype)
 
-    def forward(self, x):
-        return self._mm(x)
+    def forward(self, x, xq: Optional[NormQuant] = None):
+        return self._mm(x, xq)
 
 
 def ColumnParallelLinear(init, in_features, out_features, dtype):
@@ -225,6 +233,11 @@ class RMSNorm(nn.Module):
     def forward(self, x):
         return rms_norm(x, self.weight, self.eps)
 
+    def quant(self, x, residual=None) -> NormQuant:
+        """norm(x + residual) as an operand of the fp8 GEMMs, with the sum and the norm in x's type."""
+        return add_rms_norm_quant(x, self.weight, residual, self.eps, pow2_scale=Linear.scale_fmt == "ue8m0",
+                                  return_norm=True)
+
 
 def precompute_freqs_cis(rope_dim: int, max_seq_len: int, theta: float) -> torch.Tensor:
     inv = 1.0 / (theta**(torch.arange(0, rope_dim, 2, dtype=torch.float32) / rope_dim))
@@ -256,12 +269,12 @@ class Indexer(nn.Module):
         self.register_buffer("k_cache", torch.zeros(B, S, self.d, dtype=torch.float8_e4m3fn), persistent=False)
         self.register_buffer("k_scale", torch.zeros(B, S, dtype=torch.float32), persistent=False)
 
-    def forward(self, x, qr, start_pos, freqs):
+    def forward(self, x, qr, start_pos, freqs, xq=None, qrq=None):
         b, s, _ = x.shape
         end = start_pos + s
-        q = self.wq_b(qr).view(b, s, self.h, self.d)
+        q = self.wq_b(qr, qrq).view(b, s, self.h, self.d)
         q = torch.cat([apply_rotary_emb(q[..., :self.rope], freqs), q[..., self.rope:]], -1)
-        k = self.k_norm(self.wk(x).float()).to(x.dtype)
+        k = self.k_norm(self.wk(x, xq).float()).to(x.dtype)
         k = torch.cat([apply_rotary_emb(k[..., :self.rope], freqs), k[..., self.rope:]], -1)
         q8, qs = act_quant(q.contiguous(), group=self.d)              # [b, s, h, d], [b, s, h, 1]
         k8, ks = act_quant(k.contiguous(), group=self.d)
@@ -325,13 +338,17 @@ class MLA(nn.Module):
             self._absorb = (w[:, :self.nope].transpose(1, 2).contiguous(), w[:, self.nope:].contiguous())
         return self._absorb
 
-    def forward(self, x, start_pos, freqs):
+    def forward(self, x, start_pos, freqs, xq=None):
         b, s, _ = x.shape
         end = start_pos + s
-        qr = self.q_norm(self.wq_a(x))
-        q = self.wq_b(qr).view(b, s, self.n_local_heads, self.qk_dim)
+        if xq is None:
+            qr, qrq = self.q_norm(self.wq_a(x)), None
+        else:
+            qrq = self.q_norm.quant(self.wq_a(x, xq))
+            qr = qrq.y
+        q = self.wq_b(qr, qrq).view(b, s, self.n_local_heads, self.qk_dim)
         q_nope, q_pe = q[..., :self.nope], apply_rotary_emb(q[..., self.nope:].contiguous(), freqs)
-        kv = self.wkv_a(x)
+        kv = self.wkv_a(x, xq)
         latent, k_pe = kv[..., :self.kv_lora], kv[..., self.kv_lora:]
         self.kv_cache[:b, start_pos:end] = self.kv_norm(latent.contiguous())
         self.pe_cache[:b, start_pos:end] = apply_rotary_emb(k_pe.contiguous().unsqueeze(2), freqs).squeeze(2)
@@ -340,7 +357,7 @@ class MLA(nn.Module):
         q_lat = head_bmm(q_nope.contiguous(), w_uk_t)                           # [b, s, h, 512]
         qf = torch.cat([q_lat, q_pe], -1).contiguous()                          # [b, s, h, 576]
         kvf = torch.cat([self.kv_cache[:b, :end], self.pe_cache[:b, :end]], -1).unsqueeze(2).contiguous()
-        idx = self.indexer(x, qr, start_pos, freqs).unsqueeze(2).contiguous()    # [b, s, 1, topk]
+        idx = self.indexer(x, qr, start_pos, freqs, xq, qrq).unsqueeze(2).contiguous()    # [b, s, 1, topk]
         kern = dsa.for_target("sparse_mla_fwd", _target(x), b, s, None, self.n_local_heads, self.kv_lora, self.rope,
                               idx.shape[-1], 1, self.softmax_scale, 64, None, _tdt(x.dtype))
         o_lat, _ = kern(qf, kvf, idx)                                             # [b, s, h, 512]
@@ -364,8 +381,8 @@ class MLP(nn.Module):
         self.w3 = ColumnParallelLinear(init, dim, inter_dim, dtype)
         self.w2 = RowParallelLinear(init, inter_dim, dim, dtype, reduce_output=reduce_output)
 
-    def forward(self, x):
-        return self.w2((torch.nn.functional.silu(self.w1(x).float()) * self.w3(x).float()).to(x.dtype))
+    def forward(self, x, xq: Optional[NormQuant] = None):
+        return self.w2((torch.nn.functional.silu(self.w1(x, xq).float()) * self.w3(x, xq).float()).to(x.dtype))
 
 
 class Gate(nn.Module):
@@ -414,9 +431,11 @@ class MoE(nn.Module):
         self.w2 = nn.Parameter(w2[self.first:self.first + self.n_local].contiguous(), requires_grad=False)
         self.shared = MLP(init, H, args.n_shared_experts * F, args.dtype, reduce_output=False)
 
-    def forward(self, x):
+    def forward(self, x, xq: Optional[NormQuant] = None):
         shp = x.shape
         x = x.reshape(-1, shp[-1])
+        if xq is not None:
+            xq = xq._replace(q=xq.q.reshape(x.shape), scale=xq.scale.reshape(x.shape[0], -1))
         ids, w = self.gate(x)
         k = ids.shape[1]
         tok = torch.arange(x.shape[0], device=x.device).repeat_interleave(k)
@@ -427,7 +446,7 @@ class MoE(nn.Module):
             sel = torch.nonzero(local).squeeze(1)
             out = expert_ffn(x[tok[sel]], flat[sel] - self.first, self.w1, self.w2, self.args.block_M)
             y.index_add_(0, tok[sel], out.float() * w.reshape(-1)[sel, None])
-        y = y + self.shared(x).float()
+        y = y + self.shared(x, xq).float()
         return _all_reduce(y).to(x.dtype).reshape(shp)
 
 
@@ -440,8 +459,13 @@ class Block(nn.Module):
         self.ffn_norm = RMSNorm(args.dim, args.norm_eps, args.dtype)
         self.ffn = MLP(init, args.dim, args.inter_dim, args.dtype) if layer_id < args.n_dense_layers else \
             MoE(init, args)
+        self.fused = args.norm_quant == "fused"
 
     def forward(self, x, start_pos, freqs):
+        if self.fused:
+            n = self.attn_norm.quant(x)
+            n = self.ffn_norm.quant(self.attn(n.y, start_pos, freqs, n), x)
+            return n.h + self.ffn(n.y, n)
         x = x + self.attn(self.attn_norm(x), start_pos, freqs)
         return x + self.ffn(self.ffn_norm(x))
 
@@ -454,6 +478,10 @@ class Transformer(nn.Module):
         self.args = args
         if args.gemm_impl not in ("bf16", "fp8"):
             raise ValueError(f"gemm_impl must be 'bf16' or 'fp8', got {args.gemm_impl!r}")
+        if args.norm_quant not in ("separate", "fused"):
+            raise ValueError(f"norm_quant must be 'separate' or 'fused', got {args.norm_quant!r}")
+        if args.norm_quant == "fused" and (args.gemm_impl != "fp8" or args.dim % 128 or args.q_lora_rank % 128):
+            raise ValueError("norm_quant='fused' needs gemm_impl='fp8' and dim and q_lora_rank in groups of 128")
         Linear.fp8 = args.gemm_impl == "fp8"
         Linear.scale_fmt = args.scale_fmt
         self.embed = ParallelEmbedding(init, args.vocab_size, args.dim, args.dtype)
@@ -512,3 +540,57 @@ def generate(model: Transformer, prompt_tokens, max_new_tokens: int, temperature
         if bool(finished.all()):
             break
     return [tokens[i, prompt_lens[i]:prompt_lens[i] + max_new_tokens].tolist() for i in range(len(prompt_tokens))]
+
+
+@torch.inference_mode()
+def generate_beams(model: Transformer, prompt_tokens, max_new_tokens: int, beams: int, eos_id: int = -1):
+    """Beam search: for every prompt its ``beams`` best continuations by the sum of their log probabilities, best
+    first, as (tokens, score) pairs; a continuation ends with ``eos_id``.  Prompts of one length; the batch holds
+    ``len(prompt_tokens) * beams`` rows.
+
+    Scores, histories and caches follow their beams on the device (``beam_select``, ``reorder_states``); the host
+    waits once a step, to see whether all beams have ended, and not at all without an ``eos_id``."""
+    dev = model.freqs_cis.device
+    n, start = len(prompt_tokens), len(prompt_tokens[0])
+    if any(len(t) != start for t in prompt_tokens) or start == 0:
+        raise ValueError("generate_beams: the prompts must be of one length, and not empty")
+    if not 1 <= beams <= 32 or n * beams > model.args.max_batch_size:
+        raise ValueError(f"generate_beams: {n} prompts x {beams} beams, expected 1 to 32 beams and at most "
+                         f"max_batch_size={model.args.max_batch_size} rows")
+    total = start + max_new_tokens
+    if total > model.args.max_seq_len:
+        raise ValueError(f"generate_beams: {total} tokens, expected at most max_seq_len={model.args.max_seq_len}")
+    rows = n * beams
+    caches = []
+    for layer in model.layers:
+        a = layer.attn
+        caches += [a.kv_cache[:rows], a.pe_cache[:rows], a.indexer.k_cache[:rows], a.indexer.k_scale[:rows]]
+    tokens = torch.zeros(rows, total, dtype=torch.long, device=dev)
+    prompt = torch.tensor(prompt_tokens, dtype=torch.long, device=dev)
+    tokens[:, :start] = prompt.repeat_interleave(beams, 0)
+    scores = torch.full((n, beams), float("-inf"), device=dev)
+    scores[:, 0] = 0.0  # the beams of a prompt are still one
+    finished = torch.zeros(n, beams, dtype=torch.bool, device=dev) if eos_id >= 0 else None
+    # the prompt goes through once; its cached rows are then every beam's
+    logits = model.forward(prompt, 0).repeat_interleave(beams, 0)
+    for c in caches:
+        c = c.view(torch.uint8) if c.dtype == torch.float8_e4m3fn else c
+        c[:, :start] = c[:n, :start].repeat_interleave(beams, 0)
+    for cur in range(start, total):
+        scores, parents, nxt = beam_select(logits, scores, finished=finished, eos_id=eos_id)
+        if _world()[0] > 1:
+            for t in (scores, parents, nxt):
+                dist.broadcast(t, src=0)
+        reorder_states([tokens] + caches, parents, cur)
+        tokens[:, cur] = nxt.flatten()
+        if finished is not None:
+            finished = finished.gather(1, parents) | (nxt == eos_id)
+            if bool(finished.all()):
+                total = cur + 1
+                break
+        if cur + 1 < total:
+            logits = model.forward(tokens[:, cur:cur + 1], cur)
+    out = []
+    for row, score in zip(tokens[:, start:total].tolist(), scores.flatten().tolist()):
+        out.append((row[:row.index(eos_id) + 1] if eos_id in row else row, score))
+    return [out[i * beams:(i + 1) * beams] for i in range(n)]
