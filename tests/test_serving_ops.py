@@ -392,6 +392,25 @@ def test_attention_long(lens, new, heads, kv, dim, page):
     check_attention(q.to(FP16), c, table, lens)
 
 
+@pytest.mark.gpu
+def test_cache_beyond_32_bits():
+    """Pools of over 4 GB: the pages with the highest ids."""
+    page, heads, dim = 64, 8, 128
+    c = alloc_kv_cache(70000, heads, dim, page)
+    assert c.k.numel() > 1 << 32
+    table = torch.tensor([[69999, 2, 65600], [68000, 69998, 0]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([190, 130], dtype=torch.int32, device="cuda")
+    g = gen(9)
+    k, v = randn(g, 2, 190, heads, dim).cuda(), randn(g, 2, 190, heads, dim).cuda()
+    kv_cache_append(c, k, v, table, lens)
+    few = torch.tensor([0, 2, 65600, 68000, 69998, 69999], device="cuda")
+    small = KVCache(*(t.view(torch.uint8)[few].view(FP8) if t.dtype is FP8 else t[few] for t in c[:4]), dim)
+    near = torch.tensor([[5, 1, 2], [3, 4, 0]], dtype=torch.int32, device="cuda")
+    for new, per in ((1, 2), (40, 2)):
+        q = randn(g, 2, new, heads * per, dim).to(BF16).cuda()
+        assert torch.equal(kv_cache_attention(q, c, table, lens), check_attention(q, small, near, lens))
+
+
 @on_devices
 def test_attention_strides_scale_and_wide_table(device):
     g = gen(5)
@@ -426,11 +445,26 @@ def test_attention_absent_pages(device):
 
 
 @on_devices
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new,heads,kv,dim", [(40, 4, 1, 64), (33, 2, 2, 128), (20, 16, 2, 100), (30, 1, 1, 256)])
+def test_attention_absent_pages_in_chunks(device, page, new, heads, kv, dim):
+    """Holes of the table where every row would see the page, and where only some would."""
+    g = gen(new + dim)
+    c, table, lens = filled(g, [300, 170], kv, dim, page, device)
+    q = randn(g, 2, new, heads, dim).to(BF16).to(device)
+    t = table.clone()
+    t[0, 1], t[0, 300 // page], t[1, 170 // page] = -1, 1 << 30, -7
+    check_attention(q, c, t, lens)
+    check_attention(q.to(FP16), c, t, lens)
+
+
+@on_devices
+@pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("new,heads,dim", [(7, 2, 64), (40, 1, 128)])
-def test_attention_not_finite_in_hidden_places(device, new, heads, dim):
+def test_attention_not_finite_in_hidden_places(device, page, new, heads, dim):
     """A not-a-number in a later token's value or key reaches only the queries that see it."""
     g = gen(7)
-    n, page = 90, 16
+    n = 90
     table, pages = tables(g, [n], page)
     table, lens = table.to(device), torch.tensor([n], dtype=torch.int32, device=device)
     k, v = randn(g, 1, n, 1, dim), randn(g, 1, n, 1, dim)
@@ -555,7 +589,7 @@ def test_beam_select(device, dtype, b, k, vocab, take):
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,k,vocab,take,dtype", [
     (4, 8, 129280, 16, FP32), (1, 4, 129280, 8, FP32), (2, 16, 150001, 32, BF16), (1, 2, 32002, 64, FP16),
-    (40, 4, 32002, 8, FP16), (1, 64, 262144, 64, BF16),
+    (40, 4, 32002, 8, FP16), (1, 64, 262144, 64, BF16), (1, 3, 262145, 6, FP32), (1, 2, 1 << 20, 4, BF16),
 ])
 def test_beam_select_large(b, k, vocab, take, dtype):
     g = torch.Generator(device="cuda").manual_seed(vocab)
@@ -586,6 +620,18 @@ def test_beam_select_ties_and_not_finite(device):
     low = torch.full((1, 4, 9000), torch.finfo(FP32).min, device=device)
     check_select(low, scores, 8)
     check_select(torch.arange(9000.0, device=device).expand(1, 4, 9000), scores, 64)  # sorted, not contiguous
+
+
+@on_devices
+def test_beam_select_many_ties(device):
+    """More candidates that tie than are kept anywhere: many beams, their rows constant or of two values."""
+    zero = torch.zeros(1, 64, device=device)
+    same = torch.zeros(1, 64, 5000, device=device)
+    check_select(same, zero, 64)
+    same[:, :, ::3] = 1.0
+    check_select(same, zero, 64)
+    same[:, ::2] = -math.inf
+    check_select(same, zero, 64)
 
 
 @on_devices
