@@ -269,8 +269,7 @@ py::object kv_cache_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   if (c.cpu()) {
     tl_ops::kv_attention_cpu(a);
   } else if (out.numel()) {
-    a.splits = tl_ops::kv_attention_splits(a.batch, a.new_tokens, a.heads, a.cache.heads, a.cache.wide,
-                                           int64_t(a.cache.table_width) << a.cache.page_shift);
+    tl_ops::kv_attention_plan(a, int64_t(a.cache.table_width) << a.cache.page_shift);
     Tensor parts;  // freed on return: torch's allocator hands it out again behind this stream's work only
     if (a.splits > 1) {
       const int64_t n = batch * tokens * heads * a.splits;

@@ -39,6 +39,21 @@ __device__ inline uint32_t pack_fp8(float a, float b, float c, float d) {
   return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
 }
 
+// Eight elements that begin anywhere, as one load for 16-bit types (the memory takes any alignment), or the n that
+// there are and zeros.
+template <typename T>
+__device__ inline void load8_anywhere(const T* p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    T r[8];
+    __builtin_memcpy(r, p, sizeof(r));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = float(r[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? float(p[j]) : 0.0f;
+  }
+}
+
 template <typename F>
 __device__ inline float wave_reduce(float v, F f) {
 #pragma unroll

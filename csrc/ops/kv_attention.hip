@@ -99,6 +99,8 @@ __device__ inline void load_q(const AttentionArgs& a, int b, int head, int row, 
     const int d = 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
     if (whole) {
       q[k] = *reinterpret_cast<const X8*>(p + d);
+    } else if (row < rows && d + 8 <= c.dim) {
+      __builtin_memcpy(&q[k], p + d, sizeof(X8));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[k][j] = row < rows && d + j < c.dim ? p[d + j] : T(0.0f);
@@ -398,6 +400,10 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   }
 }
 
+// Keeps what stands before it before what stands behind it: reads of operands from LDS stay a group ahead of the
+// products that use them (4 % of the chunks' time).
+__device__ inline void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // The form for many rows (chunks of prompts): the matrix cores bound it, so the keys of a step are widened once for
 // all rows.  A workgroup holds 128 rows, 32 to a wave; waves 0-3 take the even tiles, waves 4-7 the odd ones, two
 // waves to a SIMD so that one's softmax runs beside the other's products.  Each step's two tiles lie in LDS as the
@@ -550,32 +556,51 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv_attention_chunk_kernel(At
     const int buf = step & 1, key_v = (2 * step + part) * kTile + 16 * grp;
     const Tile& t = lds.tile[buf][part];
     f32x4 s[NR][4] = {};
+    X8 k8[2][4];
 #pragma unroll
-    for (int k = 0; k < 2 * DC; ++k)
+    for (int kt = 0; kt < 4; ++kt) k8[0][kt] = t.k[kt][0][lane];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        const X8 k8 = t.k[kt][k][lane];
+    for (int k = 0; k < 2 * DC; ++k) {
+      if (k + 1 < 2 * DC) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) s[r][kt] = H::mfma(k8, q[r][k], s[r][kt]);
+        for (int kt = 0; kt < 4; ++kt) k8[(k + 1) & 1][kt] = t.k[kt][k + 1][lane];
       }
+      in_order();
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r][kt] = H::mfma(k8[k & 1][kt], q[r][k], s[r][kt]);
+      in_order();
+    }
     const Scales now = scales[buf][part][grp];
     if (MASKED) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) hide(s[r], now.there, key_v, pos[r]);
     }
     bf16x8 hi[NR][2], lo[NR][2];
+    bf16x8 v8[2][4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) v8[0][d] = t.v[d][0][lane];
+    in_order();
     softmax_step<TYPE, NR, DT, 8>(s, fmaxf(now.ks * to_log2, 1e-30f), now.vs, now.there, m, l, o, hi, lo);
+    in_order();
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+    for (int i = 0; i < 2 * DC; ++i) {  // slices 4 (i / 2) to 4 (i / 2) + 3, half i % 2 of their keys
+      if (i + 1 < 2 * DC) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bf16x8 v8 = t.v[d][u][lane];
+        for (int d = 0; d < 4; ++d) v8[(i + 1) & 1][d] = t.v[4 * ((i + 1) >> 1) + d][(i + 1) & 1][lane];
+      }
+      in_order();
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          o[r][d] = Wide::mfma(v8, hi[r][u], o[r][d]);
-          if (TYPE == kF16) o[r][d] = Wide::mfma(v8, lo[r][u], o[r][d]);
+          f32x4& to = o[r][4 * (i >> 1) + d];
+          to = Wide::mfma(v8[i & 1][d], hi[r][i & 1], to);
+          if (TYPE == kF16) to = Wide::mfma(v8[i & 1][d], lo[r][i & 1], to);
         }
-      }
+      in_order();
+    }
     const uint32_t bad = MASKED ? __builtin_amdgcn_readfirstlane(nan[buf][part]) : 0;
     if (bad) {
 #pragma unroll
@@ -592,9 +617,11 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv_attention_chunk_kernel(At
         }
       }
     }
-    write(step + 1, buf ^ 1);
-    load(step + 2, next);
-    next = pages_of(step + 3);
+    if (step + 1 < step1) {
+      write(step + 1, buf ^ 1);
+      load(step + 2, next);
+      next = pages_of(step + 3);
+    }
     __syncthreads();
   };
   // the steps whose keys all rows see
@@ -689,13 +716,9 @@ __global__ __launch_bounds__(64) void kv_join_kernel(AttentionArgs a) {
   if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// The rows of a workgroup: as few 16-row tiles as hold a key head's rows, or 128 where they are many (heads over 128
-// wide: 32, their tiles do not fit LDS twice).
-int rows_of(int rows, int wide) { return rows <= 16 ? 16 : rows <= 32 || wide > 128 ? 32 : kChunkRows; }
-
 template <Type TYPE, int DC>
 void launch_dim(const AttentionArgs& a, Stream s) {
-  const int rows = a.new_tokens * (a.heads / a.cache.heads), tile = rows_of(rows, a.cache.wide);
+  const int rows = a.new_tokens * (a.heads / a.cache.heads), tile = a.tile;
   const dim3 grid(unsigned(a.cache.heads * ceil_div(rows, tile)), a.splits, a.batch);
   const bool whole = 1 << a.cache.page_shift >= kTile;
   const char* what = "kv_cache_attention";
@@ -711,7 +734,7 @@ void launch_dim(const AttentionArgs& a, Stream s) {
   else if (tile == 32)
     launch(whole ? kv_attention_kernel<TYPE, DC, 2, true, false> : kv_attention_kernel<TYPE, DC, 2, false, false>,
            grid, kThreads, a, s, what);
-  else if constexpr (DC <= 2)
+  else if constexpr (DC == 2)
     launch(whole ? kv_attention_chunk_kernel<TYPE, DC, true> : kv_attention_chunk_kernel<TYPE, DC, false>, grid,
            kChunkThreads, a, s, what);
   if (a.splits > 1)
@@ -730,16 +753,25 @@ void launch_type(const AttentionArgs& a, Stream s) {
 
 }  // namespace
 
-// One workgroup for each of the 256 CUs, and no less than 128 keys (two waves' tiles) for each.  Measured (us, heads of
-// 128, one new token, 32 on 8 heads), by parts of the key axis:
+// Rows of a workgroup: 16 where a key head has no more, else 32, or the 128 of the chunk kernel for heads of 65 to 128
+// with enough rows and keys to fill the chip.  Its start costs 13 us against 6; measured (us, bf16, 32 heads on 8,
+// 128 rows / 32 rows, by groups of 32 rows x keys):
+//   8 x 32 tokens, 1024 keys (0.25 M) 27 / 15;   1 x 509, 2048 (1 M) 45 / 43;    4 x 509, 512 (1 M) 41 / 80
+//   2 x 509, 4096 (4 M) 88 / 123;                64 x 16, 2048 (2 M, 64 rows) 90 / 88
+// and for heads of 64, where a 32-row tile leaves room for two workgroups on a CU, 32 rows were never slower by a
+// tenth and up to 1.7 times faster.
+//
+// Parts of the key axis: one workgroup for each of the 256 CUs, and no less than 128 keys (two waves' tiles) for each.
+// Measured (us, heads of 128, one new token, 32 on 8 heads):
 //   1 x 8192 keys: 1 part 47, 8 13.9, 32 11.3, 64 13.7;      1 x 65536: 1 344, 16 35, 32 29, 64 32
 //   4 x 8192: 1 48, 4 21, 8 17, 32 22;                       32 x 8192: 1 82, 4 80, 16 107
-int kv_attention_splits(int batch, int new_tokens, int heads, int kv_heads, int wide, int64_t longest) {
-  const int rows = new_tokens * (heads / kv_heads);
-  const int64_t groups = int64_t(batch) * kv_heads * ceil_div(rows, rows_of(rows, wide));
-  int64_t parts = ceil_div(256, groups);
-  if (parts > ceil_div(longest, 2 * kTile)) parts = ceil_div(longest, 2 * kTile);
-  return int(parts < 1 ? 1 : parts > kJoinMost ? kJoinMost : parts);
+void kv_attention_plan(AttentionArgs& a, int64_t longest) {
+  const int rows = a.new_tokens * (a.heads / a.cache.heads);
+  const int64_t heads = int64_t(a.batch) * a.cache.heads;
+  a.tile = rows <= 16 ? 16 : 32;
+  if (a.cache.wide == 128 && rows > 64 && heads * ceil_div(rows, 32) * longest >= 1 << 20) a.tile = kChunkRows;
+  const int64_t parts = std::min(ceil_div(256, heads * ceil_div(rows, a.tile)), ceil_div(longest, 2 * kTile));
+  a.splits = int(std::clamp(parts, int64_t(1), int64_t(kJoinMost)));
 }
 
 void kv_attention_hip(const AttentionArgs& a, Stream s) {

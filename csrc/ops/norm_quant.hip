@@ -21,8 +21,7 @@ __device__ inline void load8(const T* p, bool whole, int n, float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = float(r[j]);
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? float(p[j]) : 0.0f;
+    load8_anywhere(p, n, v);
   }
 }
 
@@ -34,6 +33,11 @@ __device__ inline void store8(T* p, bool whole, int n, const float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = T(v[j]);
     *reinterpret_cast<V*>(p) = r;
+  } else if (n >= 8) {
+    T r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = T(v[j]);
+    __builtin_memcpy(p, r, sizeof(r));
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -41,7 +45,7 @@ __device__ inline void store8(T* p, bool whole, int n, const float (&v)[8]) {
   }
 }
 
-// WHOLE: the rows are vectors of 8 elements on 16-byte boundaries; else every element goes by itself.
+// WHOLE: the rows are vectors of 8 elements on 16-byte boundaries; else they begin and end anywhere.
 template <Type TYPE, int THREADS, int NV, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void norm_quant_kernel(NormQuantArgs a) {
   using T = typename Scalar<TYPE>::type;
@@ -120,6 +124,8 @@ __global__ __launch_bounds__(THREADS) void norm_quant_kernel(NormQuantArgs a) {
     uint8_t* q = a.q + row * width + at;
     if (WHOLE) {
       *reinterpret_cast<u32x2*>(q) = c;
+    } else if (n >= 8) {
+      __builtin_memcpy(q, &c, 8);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)

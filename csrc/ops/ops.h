@@ -76,12 +76,12 @@ struct AttentionArgs {
   int batch, new_tokens, heads;
   float scale;
   Type type;
-  int splits;     // parts of the key axis: kv_attention_splits()
-  float* part_o;  // splits > 1: [batch * new_tokens * heads, splits, dim]
-  float* part_ml; // splits > 1: [batch * new_tokens * heads, splits, 2]
+  int tile, splits;  // rows of a workgroup and parts of the key axis: kv_attention_plan()
+  float* part_o;   // splits > 1: [batch * new_tokens * heads, splits, dim]
+  float* part_ml;  // splits > 1: [batch * new_tokens * heads, splits, 2]
 };
 
-int kv_attention_splits(int batch, int new_tokens, int heads, int kv_heads, int wide, int64_t longest);
+void kv_attention_plan(AttentionArgs&, int64_t longest);  // longest: the tokens that a sequence has at most
 void kv_attention_hip(const AttentionArgs&, Stream);
 void kv_attention_cpu(const AttentionArgs&);
 

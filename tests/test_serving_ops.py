@@ -393,6 +393,51 @@ def test_attention_long(lens, new, heads, kv, dim, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lens,new,heads,kv,dim,page", [
+    ([2100, 1900] * 8, 40, 32, 8, 128, 64),  # 128 rows to a workgroup, the key axis in one part
+    ([4096, 509], 509, 32, 8, 128, 64),
+    ([3000], 700, 16, 2, 80, 16),
+    ([9000, 130], 130, 8, 2, 128, 32),
+    ([900], 300, 32, 8, 64, 16),
+    ([2000, 50], 50, 12, 2, 200, 128),
+])
+def test_attention_chunks(dtype, lens, new, heads, kv, dim, page):
+    """Prompts' chunks at full size, against float64 on the device."""
+    g = gen(sum(lens))
+    c, table, lens = filled(g, lens, kv, dim, page, "cuda")
+    q = (randn(g, len(lens), new, heads, dim) * 1.5).to(dtype).cuda()
+    got, got_lse = kv_cache_attention(q, c, table, lens, return_lse=True)
+    per = heads // kv
+    for b, n in enumerate(lens.tolist()):
+        ids = table[b, :-(-n // page)].long()
+
+        def values(pool, scale):
+            x = pool.view(torch.uint8)[ids].view(FP8).double() * scale[ids][..., None, None].double()
+            return x.transpose(0, 1)  # [head, page, ..]
+
+        k = values(c.k, c.k_scale).flatten(1, 2)[:, :n, :dim]
+        v = values(c.v, c.v_scale).transpose(2, 3).flatten(1, 2)[:, :n, :dim].contiguous()
+        x = q[b].double().view(new, kv, per, dim).permute(1, 0, 2, 3).flatten(1, 2)
+        s = (x @ k.transpose(1, 2).contiguous()) * dim**-0.5
+        size = (x.abs() @ k.abs().transpose(1, 2).contiguous()).amax(-1) * dim**-0.5
+        row = torch.arange(new, device="cuda").repeat_interleave(per)
+        hidden = torch.arange(n, device="cuda") > (n - new + row)[:, None]
+        s = s.masked_fill(hidden, -math.inf)
+        p = torch.softmax(s, -1)
+        out, bound, lse = p @ v, p @ v.abs(), torch.logsumexp(s, -1)
+        slack = 2.0**-23 * (dim + 8) * size + 1e-5
+        tol = ((2.0**-8 if dtype == BF16 else 2.0**-16) + 2 * slack[..., None]) * bound
+        tol = tol + half(dtype) * out.abs() + torch.finfo(dtype).tiny
+
+        def rows(t):
+            return t.double().unflatten(1, (kv, per)).transpose(0, 1).flatten(1, 2)
+
+        assert ((rows(got[b]) - out).abs() <= tol).all()
+        assert ((rows(got_lse[b]) - lse).abs() <= slack + 1e-6 * lse.abs()).all()
+
+
+@pytest.mark.gpu
 def test_cache_beyond_32_bits():
     """Pools of over 4 GB: the pages with the highest ids."""
     page, heads, dim = 64, 8, 128
@@ -444,6 +489,12 @@ def test_attention_absent_pages(device):
     check_attention(q, c, table, torch.tensor([(1 << 31) - 1, 97], dtype=torch.int32, device=device))
 
 
+def widened(table, page, tokens=1 << 18):
+    """The same table with room for many more tokens: a long axis is prepared for (128 rows to a workgroup, many
+    parts), whatever is there."""
+    return torch.nn.functional.pad(table, (0, tokens // page - table.shape[1]), value=-1)
+
+
 @on_devices
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("new,heads,kv,dim", [(40, 4, 1, 64), (33, 2, 2, 128), (20, 16, 2, 100), (30, 1, 1, 256)])
@@ -454,13 +505,14 @@ def test_attention_absent_pages_in_chunks(device, page, new, heads, kv, dim):
     q = randn(g, 2, new, heads, dim).to(BF16).to(device)
     t = table.clone()
     t[0, 1], t[0, 300 // page], t[1, 170 // page] = -1, 1 << 30, -7
-    check_attention(q, c, t, lens)
-    check_attention(q.to(FP16), c, t, lens)
+    for table in (t, widened(t, page)):
+        check_attention(q, c, table, lens)
+        check_attention(q.to(FP16), c, table, lens)
 
 
 @on_devices
 @pytest.mark.parametrize("page", [16, 64])
-@pytest.mark.parametrize("new,heads,dim", [(7, 2, 64), (40, 1, 128)])
+@pytest.mark.parametrize("new,heads,dim", [(7, 2, 64), (40, 1, 128), (30, 4, 100)])
 def test_attention_not_finite_in_hidden_places(device, page, new, heads, dim):
     """A not-a-number in a later token's value or key reaches only the queries that see it."""
     g = gen(7)
@@ -476,6 +528,8 @@ def test_attention_not_finite_in_hidden_places(device, page, new, heads, dim):
     c = in_use(g, pages, 1, dim, page, device)
     kv_cache_append(c, k.to(device), v.to(device), table, lens)
     q = randn(g, 1, new, heads, dim).to(BF16).to(device)
+    if heads > 2:
+        table = widened(table, page)
     want, got = kv_cache_attention(q, clean, table, lens), kv_cache_attention(q, c, table, lens)
     assert torch.equal(got[:, :new - 3], want[:, :new - 3])
     assert torch.isnan(got[:, new - 3, :, 5]).all()  # this query sees one such value
