@@ -13,6 +13,9 @@
 // beam_merge_kernel: a workgroup per sequence joins the statistics and does the same with the lists' values, which
 // are float64: there two beams' values tie only where they are equal, and within a beam they have the logits' order.
 //
+// 8 x 8 beams over 129280 fp32 logits (33 MB), 16 taken: 14 + 8 us; 4 beams over 32002 in fp16, 8 taken: 6 + 5 us.
+// The scan is one wave of workgroups, whose latency (load, threshold, exponentials, places) bounds it, not HBM.
+//
 // Where ties let too many candidates through (a constant row, say), the best one is taken `take` times instead.
 #include "device.h"
 

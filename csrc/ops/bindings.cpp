@@ -179,6 +179,7 @@ tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& 
   for (int i = 0; i < 4; ++i) c.contiguous(*all[i].first, all[i].second);
   NEED(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
        c.name, ": the cache must begin on a 16-byte boundary");
+  NEED(k.data_ptr() != v.data_ptr() && ks.data_ptr() != vs.data_ptr(), c.name, ": cache.k and cache.v share memory");
   c.dtype(table, "block_table", c10::ScalarType::Int);
   c.dims(table, "block_table", 2);
   c.size(table, "block_table", 0, batch);
@@ -381,6 +382,9 @@ void reorder_states(const std::vector<Tensor>& states, const Tensor& parents, co
   std::vector<tl_ops::ReorderState> sorted = moved;
   std::sort(sorted.begin(), sorted.end(), [](const auto& p, const auto& q) { return p.data < q.data; });
   const auto end = [&](const tl_ops::ReorderState& s) { return s.data + (rows - 1) * s.stride + s.bytes; };
+  const auto* own = static_cast<const uint8_t*>(parents.data_ptr());
+  for (const auto& t : sorted)
+    NEED(end(t) <= own || own + parents.nbytes() <= t.data, c.name, ": parents and a state share memory");
   for (size_t i = 0; i < sorted.size(); ++i)
     for (size_t j = i + 1; j < sorted.size() && sorted[j].data < end(sorted[i]); ++j) {
       const int64_t off = (sorted[j].data - sorted[i].data) % std::max<int64_t>(sorted[i].stride, 1);

@@ -95,6 +95,8 @@ def test_bitnet_generate_cached(device):
         assert (own - scores[:, k]).abs().max() < 6 * 2.0**-6
     with pytest.raises(ValueError, match="generate_cached"):
         m.generate_cached(ids, 2, beams=33)
+    with pytest.raises(ValueError, match="generate_cached"):
+        m.generate_cached(ids[:, :0], 2)
 
 
 @on_devices

@@ -589,6 +589,10 @@ def test_cache_refusals(device):
     ):
         with pytest.raises(err, match="kv_cache_append"):
             call()
+    square = alloc_kv_cache(4, 2, 64, 64, device)
+    for same in (dict(v=square.k), dict(v_scale=square.k_scale)):
+        with pytest.raises(ValueError, match="share memory"):
+            kv_cache_append(square._replace(**same), k, k, table, lens)
     for bad in ((4, 2, 257, 16), (4, 2, 0, 16), (4, 2, 64, 24), (4, 2, 64, 8)):
         with pytest.raises(ValueError, match="alloc_kv_cache"):
             alloc_kv_cache(*bad, device=device)
@@ -791,6 +795,9 @@ def test_reorder_refusals(device):
     ):
         with pytest.raises(err, match="reorder_states"):
             call()
+    with pytest.raises(ValueError, match="parents and a state share memory"):
+        q = torch.zeros(6, dtype=torch.long, device=device)
+        reorder_states([q], q.view(2, 3))
     reorder_states([], p)
 
 

@@ -207,6 +207,8 @@ class BitnetForCausalLM(nn.Module):
         b, start = input_ids.shape
         if not 1 <= beams <= 32:
             raise ValueError(f"generate_cached: {beams} beams, expected 1 to 32")
+        if start == 0:
+            raise ValueError("generate_cached: the prompts are empty")
         total = start + max_new_tokens
         rows, pages, heads = b * beams, -(-total // page_size), cfg.num_attention_heads
         caches = [alloc_kv_cache(rows * pages, heads, cfg.hidden_size // heads, page_size, dev) for _ in self.layers]
