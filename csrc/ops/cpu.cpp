@@ -71,9 +71,9 @@ void norm_quant_cpu(const NormQuantArgs& a) {
     for (int g = 0; g < a.width / a.group; ++g) {
       float m = kAmaxFloor;
       for (int j = 0; j < a.group; ++j) m = std::fmax(m, std::fabs(y[g * a.group + j]));
-      const float s = a.pow2 ? pow2_scale(m) : m / kFp8Max, inv = a.pow2 ? 1.0f / s : kFp8Max / m;
+      const float s = a.pow2 ? pow2_scale(m) : m / kFp8Max;
       a.scale[row * (a.width / a.group) + g] = s;
-      for (int j = 0; j < a.group; ++j) a.q[row * a.width + g * a.group + j] = to_fp8(y[g * a.group + j] * inv);
+      for (int j = 0; j < a.group; ++j) a.q[row * a.width + g * a.group + j] = to_fp8(y[g * a.group + j] / s);
     }
   }
 }

@@ -115,12 +115,23 @@ __global__ __launch_bounds__(THREADS) void norm_quant_kernel(NormQuantArgs a) {
     if (n <= 0) continue;
     const float m = fmaxf(amax[i], kAmaxFloor);
     const float s = a.pow2 ? pow2_scale(m) : m / kFp8Max;
-    const float inv = a.pow2 ? 1.0f / s : kFp8Max / m;
     if (at % a.group == 0) a.scale[row * groups + at / a.group] = s;
-    // no clamp: |y| inv <= 448 (1 + 2^-22), which rounds to 448
+    // y / s as IEEE division rounds it, by two corrections of y r with r = 1 / s (Markstein: where r is the rounded
+    // reciprocal and q within one last place, q + (y - q s) r rounds to the quotient; what underflows in it has the
+    // code 0).  A product with 448 / m puts 0.1 % of the codes of 16-bit rows on the other side of a tie; 8192 x 7168
+    // take 78.5 us with it, 78.9 with this and 82.0 with the compiler's division.  |y| / s rounds to 448 at most.
+    const float r = 1.0f / s, d = s < INFINITY ? s : 0.0f;  // infinite: finite values become 0, others not-a-number
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = v[i][j];
+      float q = y * r;
+      q = fmaf(fmaf(-q, d, y), r, q);
+      q = fmaf(fmaf(-q, d, y), r, q);
+      v[i][j] = copysignf(q, y);
+    }
     u32x2 c;
-    c.x = pack_fp8(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-    c.y = pack_fp8(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
+    c.x = pack_fp8(v[i][0], v[i][1], v[i][2], v[i][3]);
+    c.y = pack_fp8(v[i][4], v[i][5], v[i][6], v[i][7]);
     uint8_t* q = a.q + row * width + at;
     if (WHOLE) {
       *reinterpret_cast<u32x2*>(q) = c;

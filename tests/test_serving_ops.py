@@ -124,6 +124,40 @@ def test_norm_quant_zeros_and_not_finite(device):
 
 
 @on_devices
+@pytest.mark.parametrize("group,pow2", [(128, False), (16, False), (0, False), (128, True)])
+def test_norm_quant_codes_are_those_of_the_quotient(device, group, pow2):
+    """Rows of +1 and -1 with eps = 0: the norm's factor is 1, y the weight with a sign, both exactly, so that scale
+    and codes are what float32 divisions give (16-bit weights tie often)."""
+    g = gen(21)
+    n = 16384
+    x = (torch.randint(0, 2, (2, n), generator=g) * 2 - 1).to(BF16)
+    for dtype in (BF16, FP16, FP32):
+        w = (1 + randn(g, n) * 0.4).to(BF16).to(dtype)
+        r = add_rms_norm_quant(x.to(dtype).to(device), w.to(device), eps=0.0, group=group, pow2_scale=pow2)
+        y = (x.float() * w.float()).unflatten(1, (-1, group or n))
+        scale = y.abs().amax(-1) / 448
+        if pow2:
+            scale = torch.tensor([pow2_at_least(v) for v in scale.flatten().tolist()]).view(scale.shape)
+        assert torch.equal(r.scale.cpu(), scale)
+        want = (y / scale[..., None]).flatten(1).to(FP8)
+        assert torch.equal(codes_of(r.q.view(torch.uint8)), codes_of(want.view(torch.uint8)))
+
+
+@on_devices
+def test_norm_quant_codes_of_zeros_and_infinite_norms(device):
+    """A zero keeps its sign; a group whose largest norm is infinite has zeros beside the not-a-number."""
+    x = torch.ones(1, 256, dtype=BF16, device=device)
+    x[0, 1::2] = -1.0
+    w = torch.ones(256, device=device).to(BF16)
+    w[2:4], w[130] = 0.0, math.inf
+    r = add_rms_norm_quant(x, w, eps=0.0)
+    assert codes_of(r.q.view(torch.uint8))[0, 2:4].tolist() == [0, 0x80]
+    rest = [i for i in range(128, 256) if i != 130]
+    assert torch.isnan(r.q[0, 130].float()) and (r.q.float()[0, rest] == 0).all()
+    assert (r.q.float()[0, [0, 1]].abs() == 448).all()
+
+
+@on_devices
 def test_norm_quant_refusals(device):
     x = torch.randn(4, 256, device=device).to(BF16)
     w = torch.ones(256, dtype=BF16, device=device)
