@@ -37,6 +37,7 @@ uint8_t to_fp8(float v) { return c10::Float8_e4m3fn(v).x; }
 float from_fp8(uint8_t c) { return c10::Float8_e4m3fn(c, c10::Float8_e4m3fn::from_bits()); }
 
 float pow2_scale(float amax) {
+  if (amax == kInf) return 0x1p120f;  // that of the largest value, as the kernels take it from the bits
   int e;
   const float m = std::frexp(amax / kFp8Max, &e);
   return std::ldexp(1.0f, m == 0.5f ? e - 1 : e);

@@ -158,6 +158,17 @@ def test_norm_quant_codes_of_zeros_and_infinite_norms(device):
 
 
 @on_devices
+def test_norm_quant_infinite_norm_power_of_two(device):
+    """The group's scale is that of the largest float32, on the host as on the device."""
+    x, w = torch.ones(1, 256, dtype=BF16, device=device), torch.ones(256, dtype=BF16, device=device)
+    w[130] = math.inf
+    r = add_rms_norm_quant(x, w, eps=0.0, pow2_scale=True)
+    assert r.scale.tolist() == [[2.0**-8, 2.0**120]]
+    rest = [i for i in range(128, 256) if i != 130]
+    assert torch.isnan(r.q[0, 130].float()) and (r.q.float()[0, rest] == 0).all()
+
+
+@on_devices
 def test_norm_quant_refusals(device):
     x = torch.randn(4, 256, device=device).to(BF16)
     w = torch.ones(256, dtype=BF16, device=device)
