@@ -1,5 +1,5 @@
 // cpu.cpp -- the serving operators on host tensors: their definitions, element by element in float32 (the beam
-// search's values in float64), with the bounds checks of the device kernels.  For the models' CPU runs and tests.
+// search's values and the attention's sums in float64), with the bounds checks of the device kernels.  For the models' CPU runs and tests.
 #include <c10/util/BFloat16.h>
 #include <c10/util/Float8_e4m3fn.h>
 #include <c10/util/Half.h>
@@ -122,7 +122,8 @@ void kv_append_cpu(const AppendArgs& a) {
 void kv_attention_cpu(const AttentionArgs& a) {
   const Cache& c = a.cache;
   const int page = 1 << c.page_shift, per = a.heads / c.heads;
-  std::vector<float> q(c.dim), o(c.dim), s;
+  std::vector<float> q(c.dim), s;
+  std::vector<double> o(c.dim);  // sums of values up to float32's largest
   std::vector<int64_t> where;
   for (int b = 0; b < a.batch; ++b) {
     const int64_t len = c.lengths[b], most = int64_t(c.table_width) * page;
@@ -145,18 +146,18 @@ void kv_attention_cpu(const AttentionArgs& a) {
           where.push_back(at);
           top = std::fmax(top, s.back());
         }
-        float sum = 0.0f;
-        std::fill(o.begin(), o.end(), 0.0f);
+        double sum = 0.0;
+        std::fill(o.begin(), o.end(), 0.0);
         for (size_t j = 0; j < s.size(); ++j) {
           const float p = std::exp(s[j] - (top == -kInf ? 0.0f : top));
           const int64_t ph = page_of(c, b, where[j]) * c.heads + h / per;
           const uint8_t* v = c.v + ph * page * c.wide + where[j] % page;
           sum += p;
-          for (int d = 0; d < c.dim; ++d) o[d] += p * c.v_scale[ph] * from_fp8(v[d * page]);
+          for (int d = 0; d < c.dim; ++d) o[d] += double(p) * c.v_scale[ph] * from_fp8(v[d * page]);
         }
         const int64_t at = (int64_t(b) * a.new_tokens + i) * a.heads + h;
-        for (int d = 0; d < c.dim; ++d) store(a.out, at * c.dim + d, a.type, sum == 0.0f ? 0.0f : o[d] / sum);
-        if (a.lse) a.lse[at] = sum == 0.0f ? -kInf : top + std::log(sum);
+        for (int d = 0; d < c.dim; ++d) store(a.out, at * c.dim + d, a.type, sum == 0.0 ? 0.0f : float(o[d] / sum));
+        if (a.lse) a.lse[at] = sum == 0.0 ? -kInf : float(top + std::log(sum));
       }
   }
 }

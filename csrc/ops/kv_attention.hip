@@ -33,6 +33,9 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kTile = 64;  // keys of one wave's step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// The weighted sums of V are kept 2^32 times smaller than they are: of values up to float32's largest, 2^24 weights
+// of 2^SLACK can be summed.
+constexpr float kLogUnit = 32.0f, kUnit = 0x1p32f;
 
 // The operands of the first product: Q's type, into which e4m3 widens exactly.  (The matrix cores' own e4m3 product
 // needs no widening, with Q split into e4m3 parts; but it aligns its summands in few bits: sums of 128 were off by up
@@ -160,9 +163,9 @@ __device__ inline void softmax_step(const f32x4 (&s)[NR][4], float ks, float vs,
       for (int d = 0; d < DT; ++d) o[r][d] *= alpha;
     }
   }
-  // V's scale goes into the exponent; it is taken as 2^-100 where it is less
-  vs = fmaxf(vs, 0x1p-100f);
-  const float log_vs = __builtin_amdgcn_logf(vs), inv_vs = 1.0f / vs;
+  // V's scale goes into the exponent; it is taken as 2^-68 where it is less (an append's are 2^-22 at least)
+  vs = fmaxf(vs, 0x1p-68f);
+  const float log_vs = __builtin_amdgcn_logf(vs) - kLogUnit, inv_vs = kUnit / vs;
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     const float base = there ? log_vs - (m[r] == -INFINITY ? 0.0f : m[r]) : -INFINITY;
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
       }
       const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
       if (a.splits == 1) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : kUnit / sum;
         store4(static_cast<T*>(a.out) + out * c.dim, v * inv, d0, c.dim);
         if (d0 == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
@@ -654,7 +657,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void kv_attention_chunk_kernel(At
     const float top = fmaxf(m[r], m_lds[at]);
     const float f0 = m[r] == -INFINITY ? 0.0f : exp2_of(m[r] - top);
     const float f1 = m_lds[at] == -INFINITY ? 0.0f : exp2_of(m_lds[at] - top);
-    const float sum = l[r] * f0 + l_lds[at] * f1, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float sum = l[r] * f0 + l_lds[at] * f1, inv = sum == 0.0f ? 0.0f : kUnit / sum;
     const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
     const int64_t part_at = out * a.splits + split;
 #pragma unroll
@@ -716,7 +719,7 @@ __global__ __launch_bounds__(64) void kv_join_kernel(AttentionArgs a) {
 #pragma unroll
   for (int j = 0; j < DC; ++j)
     if (64 * j + lane < dim)
-      static_cast<T*>(a.out)[at * dim + 64 * j + lane] = T(sum == 0.0f ? 0.0f : o[j] / sum);
+      static_cast<T*>(a.out)[at * dim + 64 * j + lane] = T(sum == 0.0f ? 0.0f : o[j] / sum * kUnit);
   if (lane == 0 && a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 

@@ -595,6 +595,21 @@ def test_attention_extreme_scales(device):
 
 
 @on_devices
+@pytest.mark.parametrize("new,heads,kv", [(1, 4, 2), (24, 4, 2), (70, 4, 1)])
+def test_attention_largest_values(device, new, heads, kv):
+    """Values close to the type's largest: their weighted means are finite, the sums of many are not."""
+    g = gen(22)
+    table, pages = tables(g, [300, 90], 16)
+    table, lens = table.to(device), torch.tensor([300, 90], dtype=torch.int32, device=device)
+    c = in_use(g, pages, kv, 128, 16, device)
+    k, v = randn(g, 2, 300, kv, 128).to(BF16), (1 + torch.rand(2, 300, kv, 128, generator=g)).mul(2.0**126).to(BF16)
+    kv_cache_append(c, k.to(device), v.to(device), table, lens)
+    q = randn(g, 2, new, heads, 128).to(BF16).to(device)
+    for t in (table, widened(table, 16)):
+        assert torch.isfinite(check_attention(q, c, t, lens)).all()
+
+
+@on_devices
 def test_cache_refusals(device):
     c = alloc_kv_cache(4, 2, 64, 16, device)
     table = torch.zeros(1, 4, dtype=torch.int32, device=device)
