@@ -4,6 +4,7 @@
 // workspaces from torch's allocator on the current stream (so a call can be captured into a graph, and two calls
 // share no scratch memory) and hands plain argument blocks to the gfx950 kernels, or to their host forms for CPU
 // tensors.  Tensors of any device may be passed, whatever device is current.
+#include <ATen/EmptyTensor.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -50,8 +51,17 @@ struct Call {
     }
     NEED(t.device() == *device, name, ": argument '", arg, "' is on ", t.device().str(), ", expected ",
          device->str());
+    data(t, arg);
     if (t.requires_grad() && at::GradMode::is_enabled())
       throw std::runtime_error(text(name, ": argument '", arg, "' requires a gradient, and the operator has none"));
+  }
+  // The tensor's memory.  Fake and functional tensors, lazy zeros, wrappers and sparse ones have none.
+  void* data(const Tensor& t, const char* arg) const {
+    if (t.defined() && t.layout() == c10::kStrided && t.has_storage() && t.storage().device() == t.device()) {
+      void* const p = t.data_ptr();
+      if (p != nullptr || t.numel() == 0) return p;
+    }
+    throw py::value_error(text(name, ": argument '", arg, "' has a null data pointer"));
   }
   void dims(const Tensor& t, const char* arg, int64_t n) const {
     NEED(t.dim() == n, name, ": argument '", arg, "' has ", t.dim(), " dims, expected ", n);
@@ -81,7 +91,7 @@ struct Call {
   bool cpu() const { return device->is_cpu(); }
   // Memory of the current stream, straight from the device's allocator.
   Tensor fresh(c10::IntArrayRef sizes, c10::ScalarType s) const {
-    if (cpu()) return at::empty(sizes, at::TensorOptions().dtype(s));
+    if (cpu()) return at::detail::empty_cpu(sizes, s);
     return at::detail::empty_cuda(sizes, s, *device, c10::nullopt);
   }
   tl_ops::Stream stream() const { return c10::hip::getCurrentHIPStream(device->index()).stream(); }
@@ -133,10 +143,10 @@ py::tuple add_rms_norm_quant(const Tensor& x, const Tensor& weight, const OptTen
   const Tensor s = c.fresh(scales, c10::ScalarType::Float);
   const Tensor h = residual ? c.fresh(x.sizes(), x.scalar_type()) : Tensor();
   const Tensor y = return_norm ? c.fresh(x.sizes(), x.scalar_type()) : Tensor();
-  a.x = x2.data_ptr();
+  a.x = c.data(x2, "x");
   a.x_stride = x2.stride(0);
-  a.weight = w.data_ptr();
-  if (residual) a.residual = r2.data_ptr(), a.residual_stride = r2.stride(0), a.h = h.data_ptr();
+  a.weight = c.data(w, "weight");
+  if (residual) a.residual = c.data(r2, "residual"), a.residual_stride = r2.stride(0), a.h = h.data_ptr();
   if (return_norm) a.y = y.data_ptr();
   a.q = static_cast<uint8_t*>(q.data_ptr());
   a.scale = static_cast<float*>(s.data_ptr());
@@ -227,7 +237,7 @@ void kv_cache_append(const Tensor& k, const Tensor& v, const Tensor& ks, const T
   c10::DeviceGuard guard(*c.device);
   const Tensor x[2] = {last_dense(new_k), last_dense(new_v)};
   for (int i = 0; i < 2; ++i) {
-    a.x[i] = x[i].data_ptr();
+    a.x[i] = c.data(x[i], i ? "v" : "k");
     a.stride_b[i] = x[i].stride(0);
     a.stride_t[i] = x[i].stride(1);
     a.stride_h[i] = x[i].stride(2);
@@ -261,7 +271,7 @@ py::object kv_cache_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   c10::DeviceGuard guard(*c.device);
   const Tensor q2 = last_dense(q), out = c.fresh(q.sizes(), q.scalar_type());
   const Tensor lse = return_lse ? c.fresh({batch, tokens, heads}, c10::ScalarType::Float) : Tensor();
-  a.q = q2.data_ptr();
+  a.q = c.data(q2, "q");
   a.stride_b = q2.stride(0);
   a.stride_t = q2.stride(1);
   a.stride_h = q2.stride(2);
@@ -323,10 +333,10 @@ py::tuple beam_select(const Tensor& logits, const Tensor& scores, int64_t take, 
   const Tensor out_scores = c.fresh({batch, take}, c10::ScalarType::Float),
                out_parents = c.fresh({batch, take}, c10::ScalarType::Long),
                out_tokens = c.fresh({batch, take}, c10::ScalarType::Long);
-  a.logits = x.data_ptr();
+  a.logits = c.data(x, "logits");
   a.stride = x.stride(0);
-  a.scores = static_cast<const float*>(sc.data_ptr());
-  if (finished) a.finished = static_cast<const uint8_t*>(fin.data_ptr());
+  a.scores = static_cast<const float*>(c.data(sc, "scores"));
+  if (finished) a.finished = static_cast<const uint8_t*>(c.data(fin, "finished"));
   a.eos = eos;
   a.out_scores = static_cast<float*>(out_scores.data_ptr());
   a.out_parents = static_cast<int64_t*>(out_parents.data_ptr());

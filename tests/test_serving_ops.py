@@ -861,6 +861,45 @@ def test_reorder_refusals(device):
     reorder_states([], p)
 
 
+@on_devices
+def test_tensors_without_memory_are_refused(device):
+    """Fake, functional and batched tensors, lazy zeros, sparse ones, alone or beside real ones."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x, w = torch.randn(4, 128, device=device).to(BF16), torch.ones(128, device=device).to(BF16)
+    cache = alloc_kv_cache(2, 1, 64, 16, device)
+    table, lens = torch.zeros(1, 2, dtype=torch.int32, device=device), torch.ones(1, dtype=torch.int32, device=device)
+    kv, scores = x[:1, None, None, :64], torch.zeros(2, 2, device=device)
+    parents = torch.zeros(2, 2, dtype=torch.long, device=device)
+    calls = [("add_rms_norm_quant", lambda f: add_rms_norm_quant(f(x), w)),
+             ("add_rms_norm_quant", lambda f: add_rms_norm_quant(x, f(w))),
+             ("add_rms_norm_quant", lambda f: add_rms_norm_quant(x, w, f(x))),
+             ("kv_cache_append", lambda f: kv_cache_append(cache, f(kv), f(kv), table, lens)),
+             ("kv_cache_attention", lambda f: kv_cache_attention(f(kv), cache, table, lens)),
+             ("kv_cache_attention", lambda f: kv_cache_attention(kv, cache, table, f(lens))),
+             ("beam_select", lambda f: beam_select(f(x), scores)),
+             ("beam_select", lambda f: beam_select(x, f(scores))),
+             ("reorder_states", lambda f: reorder_states([x, f(x + 1)], parents)),
+             ("reorder_states", lambda f: reorder_states([x], f(parents)))]
+
+    def refused(call, name, f):
+        with pytest.raises((ValueError, RuntimeError), match=name):
+            call(f)
+
+    for name, call in calls:
+        mode = FakeTensorMode()
+        refused(call, name, mode.from_tensor)
+        with pytest.raises(Exception), mode:  # whatever meets the real tensors first
+            call(mode.from_tensor)
+        refused(call, name, lambda t: torch._efficientzerotensor(t.shape, dtype=t.dtype, device=device))
+        refused(call, name, lambda t: t.to_sparse())
+        torch.func.functionalize(lambda t: refused(call, name, torch._to_functional_tensor))(x)
+    for wrap in (torch.func.functionalize, torch.vmap):
+        with pytest.raises((ValueError, RuntimeError), match="null data pointer"):
+            wrap(lambda t: add_rms_norm_quant(t, w).q)(x[None] if wrap is torch.vmap else x)
+    with FakeTensorMode():  # real tensors are what they are inside such a mode
+        reorder_states([x], parents)
+
+
 # --------------------------------------------------------------------------------------------- together
 
 
