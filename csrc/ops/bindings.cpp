@@ -99,6 +99,18 @@ struct Call {
 
 Tensor last_dense(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
+// Whether the ranges of memory from the tensors' first bytes to their last ones meet.
+bool overlap(const Tensor& p, const Tensor& q) {
+  if (p.numel() == 0 || q.numel() == 0) return false;
+  const auto begin = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+  const auto end = [&](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return begin(t) + uintptr_t((last + 1) * int64_t(t.element_size()));
+  };
+  return begin(p) < end(q) && begin(q) < end(p);
+}
+
 // [..., n] as [rows, n] with dense rows
 Tensor rows_of(const Tensor& t, int64_t n) {
   return last_dense(t.dim() == 2 ? t : t.reshape({t.numel() / n, n}));
@@ -189,7 +201,6 @@ tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& 
   for (int i = 0; i < 4; ++i) c.contiguous(*all[i].first, all[i].second);
   NEED(reinterpret_cast<uintptr_t>(k.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(v.data_ptr()) % 16 == 0,
        c.name, ": the cache must begin on a 16-byte boundary");
-  NEED(k.data_ptr() != v.data_ptr() && ks.data_ptr() != vs.data_ptr(), c.name, ": cache.k and cache.v share memory");
   c.dtype(table, "block_table", c10::ScalarType::Int);
   c.dims(table, "block_table", 2);
   c.size(table, "block_table", 0, batch);
@@ -200,6 +211,9 @@ tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& 
   c.dims(lengths, "lengths", 1);
   c.size(lengths, "lengths", 0, batch);
   c.contiguous(lengths, "lengths");
+  for (int i = 1; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      NEED(!overlap(*all[i].first, *all[j].first), c.name, ": ", all[j].second, " and ", all[i].second, " share memory");
   tl_ops::Cache r{};
   r.k = static_cast<uint8_t*>(k.data_ptr());
   r.v = static_cast<uint8_t*>(v.data_ptr());
@@ -234,6 +248,14 @@ void kv_cache_append(const Tensor& k, const Tensor& v, const Tensor& ks, const T
   NEED(new_k.size(1) <= (int64_t(1) << 19), c.name, ": ", new_k.size(1), " new tokens, expected at most 2^19");
   a.batch = int(new_k.size(0));
   a.new_tokens = int(new_k.size(1));
+  // what the workgroups write must be nothing that others read
+  const std::pair<const Tensor*, const char*> read[] = {
+      {&new_k, "k"}, {&new_v, "v"}, {&table, "block_table"}, {&lengths, "lengths"}};
+  const std::pair<const Tensor*, const char*> written[] = {
+      {&k, "cache.k"}, {&v, "cache.v"}, {&ks, "cache.k_scale"}, {&vs, "cache.v_scale"}};
+  for (const auto& r : read)
+    for (const auto& w : written)
+      NEED(!overlap(*r.first, *w.first), c.name, ": ", r.second, " and ", w.second, " share memory");
   c10::DeviceGuard guard(*c.device);
   const Tensor x[2] = {last_dense(new_k), last_dense(new_v)};
   for (int i = 0; i < 2; ++i) {

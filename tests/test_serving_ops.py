@@ -658,6 +658,37 @@ def test_cache_refusals(device):
             alloc_kv_cache(*bad, device=device)
 
 
+@on_devices
+def test_cache_memory_that_is_shared(device):
+    """What a call writes may meet nothing else that it reads or writes, not by one byte."""
+    square = alloc_kv_cache(4, 2, 64, 64, device)
+    table = torch.zeros(1, 4, dtype=torch.int32, device=device)
+    lens = torch.tensor([3], dtype=torch.int32, device=device)
+    k = torch.randn(1, 1, 2, 64, device=device).to(BF16)
+    n, m = square.k.numel(), square.k_scale.numel()
+    buf = torch.zeros(2 * n + 4 * 64, dtype=torch.uint8, device=device)
+    floats = torch.ones(2 * m, device=device)
+
+    def pool(at):
+        return buf[at:at + n].view(FP8).view(4, 2, 64, 64)
+
+    def scale(at):
+        return floats[at:at + m].view(4, 2)
+
+    apart = KVCache(pool(0), pool(n), scale(0), scale(m), 64)
+    kv_cache_append(apart, k, k, table, lens)
+    tail = buf[n - 256:n].view(BF16).view(1, 1, 2, 64)  # new tokens in K's last bytes
+    ints = apart.k_scale.view(torch.int32)
+    for bad, args in ((dict(v=pool(n - 64)), ()), (dict(v=pool(0)), ()), (dict(v_scale=scale(m - 1)), ()),
+                      (dict(k_scale=buf[n - 64:n - 64 + 4 * m].view(FP32).view(4, 2)), ()),
+                      (dict(), (tail, k, table, lens)), (dict(), (k, tail, table, lens)),
+                      (dict(), (k, k, ints[:1], lens)), (dict(), (k, k, table, ints[0, :1]))):
+        with pytest.raises(ValueError, match="kv_cache_append.*share memory"):
+            kv_cache_append(apart._replace(**bad), *(args or (k, k, table, lens)))
+    with pytest.raises(ValueError, match="kv_cache_attention.*share memory"):
+        kv_cache_attention(k, apart._replace(v=pool(n - 64)), table, lens)
+
+
 # --------------------------------------------------------------------------------------------- beams
 
 

@@ -55,7 +55,8 @@ def kv_cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, block_tabl
     """Store the new tokens k, v [batch, L, kv_heads, head_dim] (bf16, fp16 or fp32, any strides) in place.
 
     ``block_table`` int32 [batch, n], ``lengths`` int32 [batch] with the new tokens counted.  Infinities are
-    stored as the page's largest value, not-a-numbers as themselves; neither sets a scale."""
+    stored as the page's largest value, not-a-numbers as themselves; neither sets a scale.  The pools and their
+    scales may share memory neither with each other nor with the call's other arguments."""
     _native.ops().kv_cache_append(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.head_dim, k, v, block_table,
                                   lengths)
 
