@@ -88,6 +88,10 @@ struct Call {
                                   ", expected BFloat16", f32 ? ", Half or Float" : " or Half"));
     }
   }
+  // `t` is about to be written: autograd has to see that what it saved of it is stale.
+  void writes(const Tensor& t) const {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
   bool cpu() const { return device->is_cpu(); }
   // Memory of the current stream, straight from the device's allocator.
   Tensor fresh(c10::IntArrayRef sizes, c10::ScalarType s) const {
@@ -256,6 +260,7 @@ void kv_cache_append(const Tensor& k, const Tensor& v, const Tensor& ks, const T
   for (const auto& r : read)
     for (const auto& w : written)
       NEED(!overlap(*r.first, *w.first), c.name, ": ", r.second, " and ", w.second, " share memory");
+  for (const auto& w : written) c.writes(*w.first);
   c10::DeviceGuard guard(*c.device);
   const Tensor x[2] = {last_dense(new_k), last_dense(new_v)};
   for (int i = 0; i < 2; ++i) {
@@ -424,6 +429,7 @@ void reorder_states(const std::vector<Tensor>& states, const Tensor& parents, co
                off + sorted[j].bytes <= sorted[i].stride,
            c.name, ": two states share memory");
     }
+  for (const Tensor& t : states) c.writes(t);
   c10::DeviceGuard guard(*c.device);
   tl_ops::ReorderArgs a{};
   a.parents = static_cast<const int64_t*>(parents.data_ptr());

@@ -931,6 +931,31 @@ def test_tensors_without_memory_are_refused(device):
         reorder_states([x], parents)
 
 
+@on_devices
+def test_writes_are_seen_by_autograd(device):
+    """A backward that saved what a call overwrites raises, instead of a gradient from the new values."""
+    g = gen(23)
+    c = alloc_kv_cache(2, 1, 64, 16, device)
+    table, lens = torch.zeros(1, 2, dtype=torch.int32, device=device), torch.ones(1, dtype=torch.int32, device=device)
+    state, k = randn(g, 4, 5).to(device), randn(g, 1, 1, 1, 64).to(device)
+    parents = torch.tensor([[1, 0], [0, 0]], device=device)
+    for saved, write in ((state, lambda: reorder_states([state], parents)),
+                         (c.k_scale, lambda: kv_cache_append(c, k, k, table, lens)),
+                         (c.v_scale, lambda: kv_cache_append(c, k, k, table, lens))):
+        w = torch.ones_like(saved, requires_grad=True)
+        y, kept = (w * saved).sum(), [(t, t._version) for t in (c.k, c.v)]
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        assert saved is state or all(t._version > v for t, v in kept)
+    with torch.inference_mode():  # these have no version to keep
+        inside = randn(g, 4, 5).to(device)
+        reorder_states([inside], parents)
+    want = inside[[0, 1, 2, 2]]
+    reorder_states([inside], torch.tensor([[0, 1], [0, 0]], device=device))
+    assert torch.equal(inside, want)
+
+
 # --------------------------------------------------------------------------------------------- together
 
 
