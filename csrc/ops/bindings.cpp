@@ -6,6 +6,7 @@
 // tensors.  Tensors of any device may be passed, whatever device is current.
 #include <ATen/EmptyTensor.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
@@ -37,7 +38,7 @@ std::string text(const A&... a) {
   } while (0)
 #define NEED(ok, ...) NEED_AS(py::value_error, ok, __VA_ARGS__)
 
-// One call's tensors: all on the first one's device, none asking for a gradient.
+// One call's tensors: all on the first one's device, none asking for a gradient or carrying a tangent.
 struct Call {
   const char* name;
   c10::optional<c10::Device> device;
@@ -54,6 +55,8 @@ struct Call {
     data(t, arg);
     if (t.requires_grad() && at::GradMode::is_enabled())
       throw std::runtime_error(text(name, ": argument '", arg, "' requires a gradient, and the operator has none"));
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+      throw std::runtime_error(text(name, ": argument '", arg, "' has a tangent, and the operator has no derivative"));
   }
   // The tensor's memory.  Fake and functional tensors, lazy zeros, wrappers and sparse ones have none.
   void* data(const Tensor& t, const char* arg) const {

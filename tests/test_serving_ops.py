@@ -956,6 +956,33 @@ def test_writes_are_seen_by_autograd(device):
     assert torch.equal(inside, want)
 
 
+@on_devices
+def test_tangents_are_refused(device):
+    """Forward-mode derivatives would be dropped: refused, as inputs that require a gradient are."""
+    import torch.autograd.forward_ad as fwAD
+    x, w, scores = torch.randn(4, 128, device=device), torch.ones(128, device=device), torch.zeros(2, 2, device=device)
+    cache = alloc_kv_cache(2, 1, 64, 16, device)
+    table, lens = torch.zeros(1, 2, dtype=torch.int32, device=device), torch.ones(1, dtype=torch.int32, device=device)
+    q, parents = x[:1, None, None, :64].to(BF16), torch.zeros(2, 2, dtype=torch.long, device=device)
+    with fwAD.dual_level():
+
+        def dual(t):
+            return fwAD.make_dual(t, torch.ones_like(t))
+
+        for name, call in (("add_rms_norm_quant", lambda: add_rms_norm_quant(dual(x), w)),
+                           ("add_rms_norm_quant", lambda: add_rms_norm_quant(x, dual(w))),
+                           ("kv_cache_append", lambda: kv_cache_append(cache, q, dual(q), table, lens)),
+                           ("kv_cache_attention", lambda: kv_cache_attention(dual(q), cache, table, lens)),
+                           ("beam_select", lambda: beam_select(dual(x), scores)),
+                           ("beam_select", lambda: beam_select(x, dual(scores))),
+                           ("reorder_states", lambda: reorder_states([dual(x)], parents))):
+            with pytest.raises(RuntimeError, match=name + ".*tangent"):
+                call()
+        with torch.inference_mode():
+            add_rms_norm_quant(dual(x), w)
+        assert add_rms_norm_quant(fwAD.unpack_dual(dual(x)).primal, w).q.shape == x.shape
+
+
 # --------------------------------------------------------------------------------------------- together
 
 

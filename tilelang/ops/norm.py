@@ -91,6 +91,7 @@ def add_rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional
     and residual of its type.  Sums and norms are float32 throughout: the codes come from the y that was not
     rounded to x's type (``rms_norm`` followed by ``act_quant`` rounds it in between).  ``h`` is returned if a
     residual is given, ``y`` with ``return_norm``.  Rows that hold infinities or not-a-numbers give
-    not-a-number codes.  No gradient: inputs that require one are refused while gradients are on.
+    not-a-number codes.  No derivative: inputs that require a gradient or carry a
+    tangent are refused while gradients are on.
     """
     return NormQuant(*_native.ops().add_rms_norm_quant(x, weight, residual, eps, group, pow2_scale, return_norm))
