@@ -53,6 +53,7 @@ struct Call {
     NEED(t.device() == *device, name, ": argument '", arg, "' is on ", t.device().str(), ", expected ",
          device->str());
     data(t, arg);
+    NEED(!t.is_neg(), name, ": argument '", arg, "' is a view whose memory holds the negative, pass its resolve_neg()");
     if (t.requires_grad() && at::GradMode::is_enabled())
       throw std::runtime_error(text(name, ": argument '", arg, "' requires a gradient, and the operator has none"));
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())

@@ -983,6 +983,18 @@ def test_tangents_are_refused(device):
         assert add_rms_norm_quant(fwAD.unpack_dual(dual(x)).primal, w).q.shape == x.shape
 
 
+@on_devices
+def test_negated_views_are_refused(device):
+    """A view that negates lazily (the imaginary part of a conjugate) would be read with the other sign."""
+    x, w = torch.randn(2, 128, device=device), torch.ones(128, device=device)
+    for call in (lambda: add_rms_norm_quant(torch._neg_view(x), w),
+                 lambda: beam_select(torch._neg_view(x), torch.zeros(1, 2, device=device))):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    got = add_rms_norm_quant(torch._neg_view(x).resolve_neg(), w)
+    assert torch.equal(got.q.float(), add_rms_norm_quant(-x, w).q.float())
+
+
 # --------------------------------------------------------------------------------------------- together
 
 
