@@ -299,6 +299,7 @@ py::object kv_cache_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   a.new_tokens = int(tokens);
   a.heads = int(heads);
   a.scale = scale ? float(*scale) : 1.0f / std::sqrt(float(dim));
+  NEED(std::isfinite(a.scale), c.name, ": sm_scale is ", *scale, ", expected a finite float32");
   c10::DeviceGuard guard(*c.device);
   const Tensor q2 = last_dense(q), out = c.fresh(q.sizes(), q.scalar_type());
   const Tensor lse = return_lse ? c.fresh({batch, tokens, heads}, c10::ScalarType::Float) : Tensor();

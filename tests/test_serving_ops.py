@@ -610,6 +610,18 @@ def test_attention_largest_values(device, new, heads, kv):
 
 
 @on_devices
+def test_attention_scale_must_be_finite(device):
+    """A not-a-number scale gave the mean of the values on the device and not-a-numbers on the host."""
+    c, table, lens = filled(gen(24), [20], 1, 64, 16, device)
+    q = randn(gen(25), 1, 1, 2, 64).to(BF16).to(device)
+    for bad in (math.nan, math.inf, -math.inf, 1e39):
+        with pytest.raises(ValueError, match="kv_cache_attention: sm_scale"):
+            kv_cache_attention(q, c, table, lens, bad)
+    check_attention(q, c, table, lens, 0.0)
+    check_attention(q, c, table, lens, 1e-30)
+
+
+@on_devices
 def test_cache_refusals(device):
     c = alloc_kv_cache(4, 2, 64, 16, device)
     table = torch.zeros(1, 4, dtype=torch.int32, device=device)
