@@ -145,10 +145,24 @@ __global__ __launch_bounds__(THREADS) void norm_quant_kernel(NormQuantArgs a) {
   }
 }
 
+// A launch has fewer than 2^32 threads: more rows than kLaunchRows take another.
+constexpr int64_t kLaunchRows = 1 << 21;
+
 template <Type TYPE, int THREADS, int NV>
 void launch_rows(const NormQuantArgs& a, bool whole, Stream s) {
-  launch(whole ? norm_quant_kernel<TYPE, THREADS, NV, true> : norm_quant_kernel<TYPE, THREADS, NV, false>,
-         dim3(unsigned(a.rows)), THREADS, a, s, "add_rms_norm_quant");
+  using T = typename Scalar<TYPE>::type;
+  for (int64_t row = 0; row < a.rows; row += kLaunchRows) {
+    NormQuantArgs part = a;
+    part.rows = a.rows - row < kLaunchRows ? a.rows - row : kLaunchRows;
+    part.x = static_cast<const T*>(a.x) + row * a.x_stride;
+    if (a.residual) part.residual = static_cast<const T*>(a.residual) + row * a.residual_stride;
+    part.q = a.q + row * a.width;
+    part.scale = a.scale + row * (a.width / a.group);
+    if (a.h) part.h = static_cast<T*>(a.h) + row * a.width;
+    if (a.y) part.y = static_cast<T*>(a.y) + row * a.width;
+    launch(whole ? norm_quant_kernel<TYPE, THREADS, NV, true> : norm_quant_kernel<TYPE, THREADS, NV, false>,
+           dim3(unsigned(part.rows)), THREADS, part, s, "add_rms_norm_quant");
+  }
 }
 
 template <Type TYPE>

@@ -168,6 +168,20 @@ def test_norm_quant_infinite_norm_power_of_two(device):
     assert torch.isnan(r.q[0, 130].float()) and (r.q.float()[0, rest] == 0).all()
 
 
+@pytest.mark.gpu
+def test_norm_quant_more_rows_than_a_launch_takes():
+    """2^26 rows of one wave each are 2^32 threads."""
+    rows, n = (1 << 26) + 5, 16
+    x = torch.empty(rows, n, dtype=BF16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    w = (1 + randn(gen(26), n) * 0.3).to(BF16).cuda()
+    r = add_rms_norm_quant(x, w, x, group=16, return_norm=True)
+    for at in (0, (1 << 21) - 2, 1 << 22, 1 << 25, rows - 4):
+        part = add_rms_norm_quant(x[at:at + 4], w, x[at:at + 4], group=16, return_norm=True)
+        check_norm(x[at:at + 4], w, x[at:at + 4], 16, False, part)
+        for got, want in zip(r, part):
+            assert torch.equal(got[at:at + 4].float(), want.float())
+
+
 @on_devices
 def test_norm_quant_refusals(device):
     x = torch.randn(4, 256, device=device).to(BF16)
