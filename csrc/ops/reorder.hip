@@ -60,18 +60,26 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(ReorderArgs a) {
 }  // namespace
 
 void reorder_hip(ReorderArgs a, Stream s) {
-  if (a.batch == 0 || a.states == 0) return;
-  int64_t blocks = 0;
-  for (int i = 0; i < a.states; ++i) {
-    a.state[i].first = blocks;
-    blocks += ceil_div(a.state[i].bytes, kBytes);
-  }
-  if (blocks > INT32_MAX) throw std::runtime_error("reorder_states: the states are too large for one call");
+  if (a.batch == 0) return;
   const auto k = a.beams <= 4    ? reorder_kernel<4>
                  : a.beams <= 8  ? reorder_kernel<8>
                  : a.beams <= 16 ? reorder_kernel<16>
                                  : reorder_kernel<32>;
-  launch(k, dim3(unsigned(blocks), unsigned(a.batch)), kThreads, a, s, "reorder_states");
+  // A launch has fewer than 2^32 threads: states whose rows are larger together take several.
+  constexpr int64_t kMost = (int64_t(1) << 32) / kThreads - 1;
+  ReorderArgs part = a;
+  for (int i = 0; i < a.states;) {
+    int64_t blocks = 0;
+    for (part.states = 0; i < a.states; ++i, ++part.states) {
+      const int64_t more = ceil_div(a.state[i].bytes, kBytes);
+      if (more > kMost) throw std::runtime_error("reorder_states: a state's row is too large");
+      if (blocks + more > kMost) break;
+      part.state[part.states] = a.state[i];
+      part.state[part.states].first = blocks;
+      blocks += more;
+    }
+    launch(k, dim3(unsigned(blocks), unsigned(a.batch)), kThreads, part, s, "reorder_states");
+  }
 }
 
 }  // namespace tl_ops

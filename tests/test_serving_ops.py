@@ -891,6 +891,26 @@ def test_reorder_many_states_and_columns(device):
         assert torch.equal(got.cpu(), ref)
 
 
+@pytest.mark.gpu
+def test_reorder_more_than_a_launch_takes():
+    """Two states of 32 GB and a little for each of two beams: 2^26 workgroups of one wave, 2^32 threads."""
+    n = (1 << 35) + 4096
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 4 * n + (8 << 30):
+        pytest.skip("needs 146 GB")
+    states = [torch.empty(2, n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    at = (0, 1 << 32, n - 64)
+    for i, s in enumerate(states):
+        for j, p in enumerate(at):
+            s[0, p:p + 64], s[1, p:p + 64] = 1, 10 * (i + 1) + j
+    reorder_states(states, torch.tensor([[1, 1]], device="cuda"))
+    for i, s in enumerate(states):
+        for j, p in enumerate(at):
+            assert (s[:, p:p + 64] == 10 * (i + 1) + j).all()
+    del states, s
+    torch.cuda.empty_cache()
+
+
 @on_devices
 def test_reorder_refusals(device):
     x, p = torch.randn(6, 10, 4, device=device), torch.zeros(2, 3, dtype=torch.long, device=device)
