@@ -304,6 +304,28 @@ def test_append(device, dtype, heads, dim, page, steps):
 
 
 @on_devices
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("heads,dim,page", [(1, 256, 128), (2, 100, 1024), (1, 192, 256), (1, 64, 512), (1, 256, 1024)])
+def test_append_large_pages(device, dtype, heads, dim, page):
+    """Pages that no workgroup holds at once: whole ones, one that ends inside, growing scales, a token alone."""
+    g = gen(dim + page)
+    steps = [([page + 37, 5], page + 37), ([page + 38, 6], 1), ([2 * page, page], page - 6), ([2 * page + 1, page + 1], 1)]
+    table, pages = tables(g, steps[-1][0], page)
+    c = in_use(g, pages, heads, dim, page, device)
+    table = table.to(device)
+    for i, (lens, new) in enumerate(steps):
+        lens = torch.tensor(lens, dtype=torch.int32)
+        k = (randn(g, 2, new, heads, dim) * 4.0**i).to(dtype)
+        v = (randn(g, 2, new, heads, dim) * 0.3 * 5.0**i).to(dtype)
+        ref = ref_append(c, k, v, table.cpu(), lens)
+        kv_cache_append(c, k.to(device), v.to(device), table, lens.to(device))
+        same_cache(c, ref)
+    for new, per in ((1, 4), (7, 3), (90, 1)):
+        q = (randn(g, 2, new, heads * per, dim) * 2).to(FP16 if dtype == FP32 else dtype).to(device)
+        check_attention(q, c, table, lens.to(device))
+
+
+@on_devices
 def test_append_values(device):
     """Infinities, not-a-numbers, zeros, values near the borders of a power of two, and strided inputs."""
     page, heads, dim = 16, 2, 64
