@@ -1,7 +1,10 @@
 """The models' paths through the serving operators: BitNet's cached decoding and beams, DeepSeek-V3.2's fused norms
 and beam search.  On the CPU (host forms) and, marked ``gpu``, on the device."""
+import os
+
 import pytest
 import torch
+import torch.multiprocessing as mp
 
 from tilelang.models import bitnet
 from tilelang.models.bitnet import BitnetConfig, BitnetForCausalLM
@@ -184,6 +187,35 @@ def test_deepseek_beam_scores():
         logits = deepseek("cpu", **one)(seqs[:, :3 + k], 0)
         total = total + torch.log_softmax(logits.double(), -1).gather(1, seqs[:, 3 + k:4 + k]).squeeze(1)
     assert (total - torch.tensor([s for _, s in got])).abs().max() < 2 * 2 * 3e-2
+
+
+def _beams_worker(rank, world, port, prompts, out):
+    import torch.distributed as dist
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        torch.save(generate_beams(deepseek("cpu", n_layers=1), prompts, 3, 3), f"{out}.{rank}")
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.timeout(600)
+def test_deepseek_beams_tensor_parallel(tmp_path):
+    """Two ranks return the same beams; their scores are the log probabilities that one process gives the tokens
+    (each logit and the normaliser within 3e-2 a step, as in test_deepseek_beam_scores)."""
+    prompts, out = [[1, 2, 3], [9, 8, 7]], str(tmp_path / "beams")
+    mp.spawn(_beams_worker, args=(2, 29500 + (os.getpid() + 977) % 2000, prompts, out), nprocs=2, join=True)
+    got = [torch.load(f"{out}.{r}", weights_only=True) for r in range(2)]
+    assert got[0] == got[1]
+    for beams in got[0]:
+        assert len(beams) == 3 and len({tuple(t) for t, _ in beams}) == 3
+        assert all(a[1] >= b[1] for a, b in zip(beams, beams[1:]))
+    seqs = torch.tensor([p + t for p, beams in zip(prompts, got[0]) for t, _ in beams])
+    total = 0.0
+    for k in range(3):
+        logp = torch.log_softmax(deepseek("cpu", n_layers=1)(seqs[:, :3 + k], 0).double(), -1)
+        total = total + logp.gather(1, seqs[:, 3 + k:4 + k]).squeeze(1)
+    assert (total - torch.tensor([s for beams in got[0] for _, s in beams])).abs().max() < 3 * 2 * 3e-2
 
 
 def test_deepseek_beams_end_and_refuse():
