@@ -218,6 +218,24 @@ def test_deepseek_beams_tensor_parallel(tmp_path):
     assert (total - torch.tensor([s for beams in got[0] for _, s in beams])).abs().max() < 3 * 2 * 3e-2
 
 
+@pytest.mark.parametrize("call", ["beams", "cached", "cached beams"])
+def test_calls_with_nothing_to_do_are_refused(call):
+    """No prompts, or fewer than one new token."""
+    if call == "beams":
+        m = deepseek("cpu", n_layers=1)
+        for prompts, new in (([], 2), ([[1, 2]], 0), ([[1, 2]], -1)):
+            with pytest.raises(ValueError, match="generate_beams"):
+                generate_beams(m, prompts, new, 2)
+        return
+    m, beams = bitnet_model("cpu"), 1 if call == "cached" else 2
+    ids = torch.zeros(1, 4, dtype=torch.long)
+    for prompts, new in ((ids[:0], 2), (ids, -1)) + (((ids, 0), ) if beams > 1 else ()):
+        with pytest.raises(ValueError, match="generate_cached"):
+            m.generate_cached(prompts, new, beams=beams)
+    if beams == 1:  # as generate
+        assert torch.equal(m.generate_cached(ids, 0), ids)
+
+
 def test_deepseek_beams_end_and_refuse():
     m = deepseek("cpu")
     first = generate(m, [[3, 1, 4]], 1)[0][0]

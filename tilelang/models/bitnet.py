@@ -207,8 +207,11 @@ class BitnetForCausalLM(nn.Module):
         b, start = input_ids.shape
         if not 1 <= beams <= 32:
             raise ValueError(f"generate_cached: {beams} beams, expected 1 to 32")
-        if start == 0:
-            raise ValueError("generate_cached: the prompts are empty")
+        if start == 0 or b == 0:
+            raise ValueError("generate_cached: the prompts are empty, or there are none")
+        if max_new_tokens < (1 if beams > 1 else 0):
+            raise ValueError(f"generate_cached: max_new_tokens is {max_new_tokens}, expected {1 if beams > 1 else 0} "
+                             "or more")
         total = start + max_new_tokens
         rows, pages, heads = b * beams, -(-total // page_size), cfg.num_attention_heads
         caches = [alloc_kv_cache(rows * pages, heads, cfg.hidden_size // heads, page_size, dev) for _ in self.layers]

@@ -551,9 +551,11 @@ def generate_beams(model: Transformer, prompt_tokens, max_new_tokens: int, beams
     Scores, histories and caches follow their beams on the device (``beam_select``, ``reorder_states``); the host
     waits once a step, to see whether all beams have ended, and not at all without an ``eos_id``."""
     dev = model.freqs_cis.device
-    n, start = len(prompt_tokens), len(prompt_tokens[0])
+    n, start = len(prompt_tokens), len(prompt_tokens[0]) if len(prompt_tokens) else 0
     if any(len(t) != start for t in prompt_tokens) or start == 0:
-        raise ValueError("generate_beams: the prompts must be of one length, and not empty")
+        raise ValueError("generate_beams: the prompts must be of one length, and not empty, nor may there be none")
+    if max_new_tokens < 1:
+        raise ValueError(f"generate_beams: max_new_tokens is {max_new_tokens}, expected 1 or more")
     if not 1 <= beams <= 32 or n * beams > model.args.max_batch_size:
         raise ValueError(f"generate_beams: {n} prompts x {beams} beams, expected 1 to 32 beams and at most "
                          f"max_batch_size={model.args.max_batch_size} rows")
