@@ -221,8 +221,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
   constexpr int ROWS = 16 * NR, DT = 4 * DC;  // rows of the workgroup, 16-wide slices of the head
   using H = Half<TYPE>;
   using X8 = typename H::X8;
-  constexpr int PASSES = NR > 2 ? 2 : 1;  // the waves join in so many passes over the head
-  constexpr int PITCH = DC * 64 / PASSES + 4;
+  constexpr int WIDTH = DC * 64, PITCH = WIDTH + 4;
   __shared__ float o_lds[kWaves][ROWS][PITCH];
   __shared__ float m_lds[kWaves][ROWS], l_lds[kWaves][ROWS];
 
@@ -369,39 +368,34 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(AttentionArgs a)
     l[r] = across_groups(l[r], Add());
     if (grp == 0) m_lds[wave][16 * r + col] = m[r], l_lds[wave][16 * r + col] = l[r];
   }
-  constexpr int WIDTH = DC * 64 / PASSES;
   const int here = rows - row0 < ROWS ? rows - row0 : ROWS;
 #pragma unroll
-  for (int pass = 0; pass < PASSES; ++pass) {
-    if (pass) __syncthreads();
+  for (int r = 0; r < NR; ++r)
 #pragma unroll
-    for (int r = 0; r < NR; ++r)
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<f32x4*>(&o_lds[wave][16 * r + col][16 * d + 4 * grp]) = o[r][d];
+  __syncthreads();
+  for (int i = threadIdx.x; i < here * (WIDTH / 4); i += kThreads) {
+    const int r = i / (WIDTH / 4), d0 = i % (WIDTH / 4) * 4, row = row0 + r;
+    float top = m_lds[0][r], sum = 0.0f;
 #pragma unroll
-      for (int d = 0; d < DT / PASSES; ++d)
-        *reinterpret_cast<f32x4*>(&o_lds[wave][16 * r + col][16 * d + 4 * grp]) = o[r][pass * (DT / PASSES) + d];
-    __syncthreads();
-    for (int i = threadIdx.x; i < here * (WIDTH / 4); i += kThreads) {
-      const int r = i / (WIDTH / 4), d4 = i % (WIDTH / 4) * 4, d0 = pass * WIDTH + d4, row = row0 + r;
-      float top = m_lds[0][r], sum = 0.0f;
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][r]);
+    f32x4 v = {};
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][r]);
-      f32x4 v = {};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = m_lds[w][r] == -INFINITY ? 0.0f : exp2_of(m_lds[w][r] - top);
-        sum += l_lds[w][r] * f;
-        v += *reinterpret_cast<const f32x4*>(&o_lds[w][r][d4]) * f;
-      }
-      const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
-      if (a.splits == 1) {
-        const float inv = sum == 0.0f ? 0.0f : kUnit / sum;
-        store4(static_cast<T*>(a.out) + out * c.dim, v * inv, d0, c.dim);
-        if (d0 == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-      } else {
-        const int64_t part = out * a.splits + split;
-        store4(a.part_o + part * c.dim, v, d0, c.dim);
-        if (d0 == 0) a.part_ml[part * 2] = top, a.part_ml[part * 2 + 1] = sum;
-      }
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = m_lds[w][r] == -INFINITY ? 0.0f : exp2_of(m_lds[w][r] - top);
+      sum += l_lds[w][r] * f;
+      v += *reinterpret_cast<const f32x4*>(&o_lds[w][r][d0]) * f;
+    }
+    const int64_t out = (int64_t(b) * a.new_tokens + row / per) * a.heads + head * per + row % per;
+    if (a.splits == 1) {
+      const float inv = sum == 0.0f ? 0.0f : kUnit / sum;
+      store4(static_cast<T*>(a.out) + out * c.dim, v * inv, d0, c.dim);
+      if (d0 == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    } else {
+      const int64_t part = out * a.splits + split;
+      store4(a.part_o + part * c.dim, v, d0, c.dim);
+      if (d0 == 0) a.part_ml[part * 2] = top, a.part_ml[part * 2 + 1] = sum;
     }
   }
 }
