@@ -54,6 +54,7 @@ struct Call {
          device->str());
     data(t, arg);
     NEED(!t.is_neg(), name, ": argument '", arg, "' is a view whose memory holds the negative, pass its resolve_neg()");
+    if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return;
     if (t.requires_grad() && at::GradMode::is_enabled())
       throw std::runtime_error(text(name, ": argument '", arg, "' requires a gradient, and the operator has none"));
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
@@ -107,16 +108,18 @@ struct Call {
 
 Tensor last_dense(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
-// Whether the ranges of memory from the tensors' first bytes to their last ones meet.
-bool overlap(const Tensor& p, const Tensor& q) {
-  if (p.numel() == 0 || q.numel() == 0) return false;
-  const auto begin = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
-  const auto end = [&](const Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return begin(t) + uintptr_t((last + 1) * int64_t(t.element_size()));
-  };
-  return begin(p) < end(q) && begin(q) < end(p);
+// The memory from a tensor's first byte to its last one.
+struct Range {
+  uintptr_t begin, end;
+  bool meets(const Range& r) const { return begin < r.end && r.begin < end; }
+};
+Range range_of(const Tensor& t) {
+  const auto begin = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {begin, 0};  // meets nothing
+  const auto sizes = t.sizes(), strides = t.strides();
+  int64_t last = 0;
+  for (size_t d = 0; d < sizes.size(); ++d) last += (sizes[d] - 1) * strides[d];
+  return {begin, begin + uintptr_t((last + 1) * int64_t(t.element_size()))};
 }
 
 // [..., n] as [rows, n] with dense rows
@@ -181,7 +184,7 @@ py::tuple add_rms_norm_quant(const Tensor& x, const Tensor& weight, const OptTen
 // ------------------------------------------------------------------------------------------- cache
 
 tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t dim,
-                       const Tensor& table, const Tensor& lengths, int64_t batch) {
+                       const Tensor& table, const Tensor& lengths, int64_t batch, Range (&pools)[4]) {
   const std::pair<const Tensor*, const char*> all[] = {{&k, "cache.k"},             {&v, "cache.v"},
                                                        {&ks, "cache.k_scale"},      {&vs, "cache.v_scale"},
                                                        {&table, "block_table"},     {&lengths, "lengths"}};
@@ -219,9 +222,11 @@ tl_ops::Cache cache_of(Call& c, const Tensor& k, const Tensor& v, const Tensor& 
   c.dims(lengths, "lengths", 1);
   c.size(lengths, "lengths", 0, batch);
   c.contiguous(lengths, "lengths");
-  for (int i = 1; i < 4; ++i)
+  for (int i = 0; i < 4; ++i) {
+    pools[i] = range_of(*all[i].first);
     for (int j = 0; j < i; ++j)
-      NEED(!overlap(*all[i].first, *all[j].first), c.name, ": ", all[j].second, " and ", all[i].second, " share memory");
+      NEED(!pools[i].meets(pools[j]), c.name, ": ", all[j].second, " and ", all[i].second, " share memory");
+  }
   tl_ops::Cache r{};
   r.k = static_cast<uint8_t*>(k.data_ptr());
   r.v = static_cast<uint8_t*>(v.data_ptr());
@@ -249,7 +254,8 @@ void kv_cache_append(const Tensor& k, const Tensor& v, const Tensor& ks, const T
   a.type = c.type(new_k, "k", true);
   c.dtype(new_v, "v", new_k.scalar_type());
   NEED(new_v.sizes() == new_k.sizes(), c.name, ": v ", new_v.sizes(), " does not match k ", new_k.sizes());
-  a.cache = cache_of(c, k, v, ks, vs, dim, table, lengths, new_k.size(0));
+  Range pools[4];
+  a.cache = cache_of(c, k, v, ks, vs, dim, table, lengths, new_k.size(0), pools);
   c.size(new_k, "k", 2, a.cache.heads);
   c.size(new_k, "k", 3, dim);
   NEED(new_k.size(0) <= 32767, c.name, ": ", new_k.size(0), " sequences, expected at most 32767");
@@ -261,9 +267,11 @@ void kv_cache_append(const Tensor& k, const Tensor& v, const Tensor& ks, const T
       {&new_k, "k"}, {&new_v, "v"}, {&table, "block_table"}, {&lengths, "lengths"}};
   const std::pair<const Tensor*, const char*> written[] = {
       {&k, "cache.k"}, {&v, "cache.v"}, {&ks, "cache.k_scale"}, {&vs, "cache.v_scale"}};
-  for (const auto& r : read)
-    for (const auto& w : written)
-      NEED(!overlap(*r.first, *w.first), c.name, ": ", r.second, " and ", w.second, " share memory");
+  for (const auto& r : read) {
+    const Range range = range_of(*r.first);
+    for (int i = 0; i < 4; ++i)
+      NEED(!range.meets(pools[i]), c.name, ": ", r.second, " and ", written[i].second, " share memory");
+  }
   for (const auto& w : written) c.writes(*w.first);
   c10::DeviceGuard guard(*c.device);
   const Tensor x[2] = {last_dense(new_k), last_dense(new_v)};
@@ -287,7 +295,8 @@ py::object kv_cache_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   c.dims(q, "q", 4);
   tl_ops::AttentionArgs a{};
   a.type = c.type(q, "q", false);
-  a.cache = cache_of(c, k, v, ks, vs, dim, table, lengths, q.size(0));
+  Range pools[4];
+  a.cache = cache_of(c, k, v, ks, vs, dim, table, lengths, q.size(0), pools);
   c.size(q, "q", 3, dim);
   const int64_t batch = q.size(0), tokens = q.size(1), heads = q.size(2);
   NEED(heads >= 1 && heads % a.cache.heads == 0, c.name, ": ", heads, " query heads do not share ", a.cache.heads,
