@@ -11,7 +11,10 @@
 // the lanes' maxima, found bit by bit with one ballot each, few logits reach T.  Those go to LDS, and each finds its
 // place by counting the larger ones.
 // beam_merge_kernel: a workgroup per sequence joins the statistics and does the same with the lists' values, which
-// are float64: there two beams' values tie only where they are equal, and within a beam they have the logits' order.
+// are float64: within a beam they have the logits' order.  A beam's logsumexp comes from float32 exponentials and
+// sums of each wave, joined in float64: off by less than 2^-19 (a term 2^-d of the largest by d 2^-23 of itself, and d
+// is 20 on average at most), which can decide between two beams' values that are as close; float64 exponentials of
+// every logit would cost more than the scan does.
 //
 // 8 x 8 beams over 129280 fp32 logits (33 MB), 16 taken: 14 + 8 us; 4 beams over 32002 in fp16, 8 taken: 6 + 5 us.
 // The scan is one wave of workgroups, whose latency (load, threshold, exponentials, places) bounds it, not HBM.

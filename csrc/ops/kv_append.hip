@@ -3,10 +3,17 @@
 //   s_new = pow2ceil(max |new tokens of the page| / 448);  s = s_new if the page begins with them, else
 //   max(s_old, s_new);  codes = e4m3(x / s), and the page's older codes c become e4m3(c s_old / s) if s grew.
 //
-// Scales are powers of two: dividing by one rounds nothing, so a code that is scaled again keeps its value but for
-// what falls below e4m3's smallest step.  One workgroup owns one (page, head) of K or of V: no two write one scale.
+// Scales are powers of two: a code that is scaled again keeps its value unless it becomes subnormal.  Then it is
+// rounded once more, to a multiple of 2^-9 of the new scale: off by up to 2^-10 of it, each time.  One workgroup owns
+// one (page, head) of K or of V: no two write one scale.
 //
-// Bound by HBM: 3 bytes an element in 16 bits.  8 prompts of 4001 tokens, 8 heads of 128 (197 MB): 42 us, 4.7 TB/s.
+// Bound by HBM: 3 bytes an element in 16 bits.  8 prompts of 4001 tokens, 8 heads of 128 (197 MB): 40 us, 4.9 TB/s;
+// pages of over 512 items (KEEP = false) read their tokens a second time: heads of 256 in pages of 128 2.5 times a
+// copy's time, pages of 1024 2.2 times.
+//
+// Codes that are scaled again take a read and a write of one byte for each thread in turn, which bounds the calls that
+// reach it: one token for 32 sequences, 8 heads of 128, pages of 64 that are nearly full, in a graph, 48 us where every
+// scale grows against 5.7 where none does; pages of 1024 tokens of 256 1.4 ms.
 #include "device.h"
 
 namespace tl_ops {
@@ -93,7 +100,7 @@ __global__ __launch_bounds__(THREADS) void kv_append_kernel(AppendArgs a) {
   if (tid == 0) *scale_at = scale;
 
   // A whole page of V turns around in LDS and is written in its own order (up to 256 rows, padded by a dword
-  // against bank conflicts): 42 us for 8 x 4001 tokens in 8 heads of 128, 49 with each thread's dwords straight to
+  // against bank conflicts): 40 us for 8 x 4001 tokens in 8 heads of 128, 48 with each thread's dwords straight to
   // memory.
   __shared__ uint32_t tile[TILE ? THREADS * kDims + 256 : 1];
   const bool whole = TILE && which && s.n == page;

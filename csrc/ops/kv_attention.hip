@@ -13,13 +13,16 @@
 // K's contraction goes over d = 64 chunk + 16 g + 0..15 for the same reason: both operands come from memory in
 // 16-byte loads and the softmax needs one exchange over the four lane groups.  e4m3 widens to bf16 and fp16 exactly;
 // the products run on 16-bit operands and accumulate in float32.  P is rounded to bf16 (V's scale folded in, whose
-// range only bf16 has); for fp16 the rounding's rest goes through a second product, which keeps the error that of
-// the output's own rounding.
+// range only bf16 has): a weight is off by up to 2^-8 of itself, as the output's own rounding to bf16 is of it.  The
+// largest weight is 1 and exact here, which leaves the error against float64 that of the output's rounding (0.0017 in
+// the root mean square, 32 sequences of up to 8192 keys); for the chunks see SLACK.  For fp16 the rounding's rest goes
+// through a second product, which keeps the error that of the output's own rounding there too.
 //
 // The waves of a workgroup take tiles in turn and join in LDS; `splits` workgroups share a long key axis and
 // kv_join_kernel joins them (3 us for 32 rows in 7 parts).
 //
-// Single tokens are bound by HBM: no byte of the cache is read twice, and two workgroups on a CU keep 128 KB in flight.
+// Single tokens are bound by HBM: no byte of the cache is read twice, and two workgroups on a CU (heads up to 128; wider
+// ones have registers for one) keep 128 KB in flight.
 // 32 sequences of 4096 to 8192 tokens, 32 heads on 8 of 128: 75 us, 5.4 TB/s; one of 777 tokens: 6.4 us and the join.
 #include <algorithm>
 #include <type_traits>
@@ -137,7 +140,9 @@ __device__ inline void poison(bf16x8 is, bool there, int key, int pos, f32x4& o)
 // The weights of 16 scores of each of NR rows (in units of 1 / ks), with V's scale, as operands of the second
 // product; a page that is not `there` has none.  The sums are relative to m, which moves when the scores outgrow it by
 // more than a factor of 2^SLACK.  With 0 the largest weight is 1 and rounds to itself; a larger one saves most of the
-// sums' rescaling where that counts (weights up to 2^SLACK fit bf16 and float32 as well).
+// sums' rescaling where that counts, and rounds the largest weight too.  2 x 509 tokens on up to 4096 keys in the chunk
+// form: 82.0 us and an error against float64 of 0.0021 with 8, 86.7 us and 0.0018 with 0, of which the output's
+// rounding is 0.0017.
 template <Type TYPE, int NR, int DT, int SLACK>
 __device__ inline void softmax_step(const f32x4 (&s)[NR][4], float ks, float vs, bool there, float (&m)[NR],
                                     float (&l)[NR], f32x4 (&o)[NR][DT], bf16x8 (&hi)[NR][2], bf16x8 (&lo)[NR][2]) {
@@ -760,7 +765,10 @@ void launch_type(const AttentionArgs& a, Stream s) {
 //   8 x 32 tokens, 1024 keys (0.25 M) 27 / 15;   1 x 509, 2048 (1 M) 45 / 43;    4 x 509, 512 (1 M) 41 / 80
 //   2 x 509, 4096 (4 M) 88 / 123;                64 x 16, 2048 (2 M, 64 rows) 90 / 88
 // and for heads of 64, where a 32-row tile leaves room for two workgroups on a CU, 32 rows were never slower by a
-// tenth and up to 1.7 times faster.
+// tenth and up to 1.7 times faster.  Heads of 129 to 256 have no other form for many rows; it fills the registers (at
+// 256 wide 63 to 81 go to scratch memory): 2 x 509 tokens on up to 4096 keys take 170 us at 192 wide and 349 at 256.
+// Rows and parts come from what the table can hold, since the lengths are the device's: 20 tokens on 777 keys take
+// 13.5 us, and 20.3 with a table for 65536.
 //
 // Parts of the key axis: one workgroup for each of the 256 CUs, and no less than 128 keys (two waves' tiles) for each.
 // Measured (us, heads of 128, one new token, 32 on 8 heads):

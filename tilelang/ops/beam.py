@@ -22,7 +22,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: Optional[int] 
 
         scores[k] + logits[k, t] - logsumexp(logits[k])
 
-    in float64, and the largest come first, ties by the lowest ``k * vocab + t``.  A beam of ``finished`` [batch,
+    in float64 but for the logsumexp, which float32 exponentials and sums give on the device (off by less than
+    2^-19), and the largest come first, ties by the lowest ``k * vocab + t``.  One beam's tokens are always in the
+    order of their logits; between two beams, values that are closer than that may come in either order.  A beam of ``finished`` [batch,
     beams] (bool) has one continuation, ``eos_id``, with its score as it is.  Not-a-number values count as -inf, so
     a beam whose logits hold not-a-numbers or +inf, or whose score is not finite, comes last.
 

@@ -11,7 +11,8 @@ The layout is made for the attention kernel (csrc/ops/kv_attention.hip): K pages
 [dim, token], both head-major, the head padded with zeros to a multiple of 64.
 
 * Scales are powers of two.  When a new token is larger than its page's scale allows, the page's codes are scaled
-  again, which loses nothing but what falls below e4m3's smallest step.  The first token of a page sets its scale
+  again: exactly, but for values that become subnormal in e4m3, which are rounded once more, by up to 2^-10 of the
+  new scale each time.  The first token of a page sets its scale
   anew, whatever the page held before.
 * A page that sequences share may be read by all of them; only one may append to it in a call.
 * Page ids outside the pool (a table padded with -1, say) are not followed: their tokens are not stored, and count

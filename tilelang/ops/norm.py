@@ -90,8 +90,9 @@ def add_rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional
     of two from 16 to 512 that divides the row.  x [..., N] in bf16, fp16 or fp32 (N up to 65536) with weight [N]
     and residual of its type.  Sums and norms are float32 throughout: the codes come from the y that was not
     rounded to x's type (``rms_norm`` followed by ``act_quant`` rounds it in between).  ``h`` is returned if a
-    residual is given, ``y`` with ``return_norm``.  Rows that hold infinities or not-a-numbers give
-    not-a-number codes.  No derivative: inputs that require a gradient or carry a
+    residual is given, ``y`` with ``return_norm``.  A row with a not-a-number has
+    not-a-number codes; one whose squares sum to more than float32 holds (an infinite element, say) has zeros, and
+    not-a-number at an infinite element.  No derivative: inputs that require a gradient or carry a
     tangent are refused while gradients are on.
     """
     return NormQuant(*_native.ops().add_rms_norm_quant(x, weight, residual, eps, group, pow2_scale, return_norm))
