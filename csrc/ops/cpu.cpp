@@ -1,5 +1,6 @@
 // cpu.cpp -- the serving operators on host tensors: their definitions, element by element in float32 (the beam
-// search's values and the attention's sums in float64), with the bounds checks of the device kernels.  For the models' CPU runs and tests.
+// search's values and the attention's sums in float64), with the bounds checks of the device kernels.  For the models'
+// CPU runs and tests.
 #include <c10/util/BFloat16.h>
 #include <c10/util/Float8_e4m3fn.h>
 #include <c10/util/Half.h>

@@ -21,8 +21,8 @@
 // The waves of a workgroup take tiles in turn and join in LDS; `splits` workgroups share a long key axis and
 // kv_join_kernel joins them (3 us for 32 rows in 7 parts).
 //
-// Single tokens are bound by HBM: no byte of the cache is read twice, and two workgroups on a CU (heads up to 128; wider
-// ones have registers for one) keep 128 KB in flight.
+// Single tokens are bound by HBM: no byte of the cache is read twice, and two workgroups on a CU (heads up to 128;
+// wider ones have registers for one) keep 128 KB in flight.
 // 32 sequences of 4096 to 8192 tokens, 32 heads on 8 of 128: 75 us, 5.4 TB/s; one of 777 tokens: 6.4 us and the join.
 #include <algorithm>
 #include <type_traits>

@@ -309,7 +309,8 @@ def test_append(device, dtype, heads, dim, page, steps):
 def test_append_large_pages(device, dtype, heads, dim, page):
     """Pages that no workgroup holds at once: whole ones, one that ends inside, growing scales, a token alone."""
     g = gen(dim + page)
-    steps = [([page + 37, 5], page + 37), ([page + 38, 6], 1), ([2 * page, page], page - 6), ([2 * page + 1, page + 1], 1)]
+    steps = [([page + 37, 5], page + 37), ([page + 38, 6], 1), ([2 * page, page], page - 6),
+             ([2 * page + 1, page + 1], 1)]
     table, pages = tables(g, steps[-1][0], page)
     c = in_use(g, pages, heads, dim, page, device)
     table = table.to(device)

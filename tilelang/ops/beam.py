@@ -23,10 +23,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, take: Optional[int] 
         scores[k] + logits[k, t] - logsumexp(logits[k])
 
     in float64 but for the logsumexp, which float32 exponentials and sums give on the device (off by less than
-    2^-19), and the largest come first, ties by the lowest ``k * vocab + t``.  One beam's tokens are always in the
-    order of their logits; between two beams, values that are closer than that may come in either order.  A beam of ``finished`` [batch,
-    beams] (bool) has one continuation, ``eos_id``, with its score as it is.  Not-a-number values count as -inf, so
-    a beam whose logits hold not-a-numbers or +inf, or whose score is not finite, comes last.
+    2^-19), and the largest come first, ties by the lowest ``k * vocab + t``. One beam's tokens are always in the
+    order of their logits; between two beams, values that are closer than that may come in either order. A beam of
+    ``finished`` [batch, beams] (bool) has one continuation, ``eos_id``, with its score as it is. Not-a-number
+    values count as -inf, so a beam whose logits hold not-a-numbers or +inf, or whose score is not finite, comes
+    last.
 
     Returns (scores float32, parents int64, tokens int64), each [batch, take]."""
     return _native.ops().beam_select(logits, scores, scores.shape[-1] if take is None else take, finished, eos_id)

@@ -10,10 +10,11 @@ left): they are not stored, and their queries give zeros.
 The layout is made for the attention kernel (csrc/ops/kv_attention.hip): K pages are [token, dim], V pages
 [dim, token], both head-major, the head padded with zeros to a multiple of 64.
 
-* Scales are powers of two.  When a new token is larger than its page's scale allows, the page's codes are scaled
+* Scales are powers of two. When a new token is larger than its page's scale allows, the page's codes are scaled
   again: exactly, but for values that become subnormal in e4m3, which are rounded once more, by up to 2^-10 of the
-  new scale each time.  The first token of a page sets its scale
-  anew, whatever the page held before.
+  new scale each time. The first token of a page sets its scale anew, whatever the page held before. Scales of an
+  append are 2^-22 at least; pools that a caller fills may hold V scales down to 2^-68 (a smaller one counts as
+  that).
 * A page that sequences share may be read by all of them; only one may append to it in a call.
 * Page ids outside the pool (a table padded with -1, say) are not followed: their tokens are not stored, and count
   as absent for the attention.  So do tokens beyond the table.

@@ -86,13 +86,12 @@ def add_rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional
 
         scale = max(max |y|, 1e-4) / 448, or the next power of two (``pow2_scale``);  q = e4m3(y / scale)
 
-    the operand format of ``fp8_gemm`` for ``group=128``.  ``group=0``: one scale for each row; otherwise a power
-    of two from 16 to 512 that divides the row.  x [..., N] in bf16, fp16 or fp32 (N up to 65536) with weight [N]
-    and residual of its type.  Sums and norms are float32 throughout: the codes come from the y that was not
-    rounded to x's type (``rms_norm`` followed by ``act_quant`` rounds it in between).  ``h`` is returned if a
-    residual is given, ``y`` with ``return_norm``.  A row with a not-a-number has
-    not-a-number codes; one whose squares sum to more than float32 holds (an infinite element, say) has zeros, and
-    not-a-number at an infinite element.  No derivative: inputs that require a gradient or carry a
-    tangent are refused while gradients are on.
+    the operand format of ``fp8_gemm`` for ``group=128``. ``group=0``: one scale for each row; otherwise a power of
+    two from 16 to 512 that divides the row. x [..., N] in bf16, fp16 or fp32 (N up to 65536) with weight [N] and
+    residual of its type. Sums and norms are float32 throughout: the codes come from the y that was not rounded to
+    x's type (``rms_norm`` followed by ``act_quant`` rounds it in between). ``h`` is returned if a residual is
+    given, ``y`` with ``return_norm``. A row with a not-a-number has not-a-number codes; one whose squares sum to
+    more than float32 holds (an infinite element, say) has zeros, and not-a-number at an infinite element. No
+    derivative: inputs that require a gradient or carry a tangent are refused while gradients are on.
     """
     return NormQuant(*_native.ops().add_rms_norm_quant(x, weight, residual, eps, group, pow2_scale, return_norm))
