@@ -426,6 +426,8 @@ void reorder_states(const std::vector<Tensor>& states, const Tensor& parents, co
     const int64_t bytes = moves * int64_t(t.element_size()), stride = t.stride(0) * int64_t(t.element_size());
     if (bytes == 0) continue;
     NEED(rows == 1 || stride >= bytes, c.name, ": a state's rows overlap");
+    NEED(bytes <= tl_ops::kReorderMaxBytes, c.name, ": ", bytes, " bytes of a state's row, expected at most ",
+         tl_ops::kReorderMaxBytes);
     moved.push_back({static_cast<uint8_t*>(t.data_ptr()), stride, bytes, 0});
   }
   // No byte may be moved twice.  In the order of their addresses, two states that share a range must be columns of

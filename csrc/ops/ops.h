@@ -123,6 +123,8 @@ struct ReorderState {
 
 constexpr int kReorderMaxBeams = 32;
 constexpr int kReorderStates = 96;  // states that one launch takes
+// and bytes of their rows: a wave moves 1024 of them, and a launch has fewer than 2^32 threads
+constexpr int64_t kReorderMaxBytes = (int64_t(1) << 36) - 1024;
 
 struct ReorderArgs {
   ReorderState state[kReorderStates];

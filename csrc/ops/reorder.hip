@@ -66,14 +66,14 @@ void reorder_hip(ReorderArgs a, Stream s) {
                  : a.beams <= 8  ? reorder_kernel<8>
                  : a.beams <= 16 ? reorder_kernel<16>
                                  : reorder_kernel<32>;
-  // A launch has fewer than 2^32 threads: states whose rows are larger together take several.
-  constexpr int64_t kMost = (int64_t(1) << 32) / kThreads - 1;
+  // States whose rows are larger together than a launch takes go into several.
+  constexpr int64_t kMost = kReorderMaxBytes / kBytes;
+  static_assert((kMost + 1) * kThreads == int64_t(1) << 32);
   ReorderArgs part = a;
   for (int i = 0; i < a.states;) {
     int64_t blocks = 0;
     for (part.states = 0; i < a.states; ++i, ++part.states) {
       const int64_t more = ceil_div(a.state[i].bytes, kBytes);
-      if (more > kMost) throw std::runtime_error("reorder_states: a state's row is too large");
       if (blocks + more > kMost) break;
       part.state[part.states] = a.state[i];
       part.state[part.states].first = blocks;

@@ -934,6 +934,22 @@ def test_reorder_more_than_a_launch_takes():
     torch.cuda.empty_cache()
 
 
+def test_reorder_rows_that_no_launch_takes(tmp_path):
+    """Refused before anything moves: rows of 2^36 bytes, in a sparse file that nobody reads or writes."""
+    n = 1 << 36
+    try:
+        with open(tmp_path / "state", "wb") as f:
+            f.truncate(2 * n)
+        huge = torch.from_file(str(tmp_path / "state"), shared=True, size=2 * n, dtype=torch.uint8).view(2, n)
+    except (OSError, RuntimeError) as e:
+        pytest.skip(f"no sparse file of 128 GB here: {e}")
+    small = torch.arange(2.0).view(2, 1)
+    with pytest.raises(ValueError, match="reorder_states: 68719476736 bytes of a state's row"):
+        reorder_states([small, huge], torch.tensor([[1, 1]]))
+    assert small.tolist() == [[0.0], [1.0]]
+    reorder_states([small, huge], torch.tensor([[1, 1]]), 1)  # what moves of a row counts
+
+
 @on_devices
 def test_reorder_refusals(device):
     x, p = torch.randn(6, 10, 4, device=device), torch.zeros(2, 3, dtype=torch.long, device=device)

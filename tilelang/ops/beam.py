@@ -38,6 +38,6 @@ def reorder_states(states: Sequence[torch.Tensor], parents: torch.Tensor, length
 
     Each state is [batch * beams, ...] of any type; parents int64 [batch, beams] within a sequence (a parent outside
     0 .. beams - 1 leaves its beam as it is; at most 32 beams).  ``length``: only the first ``length`` entries of
-    the states' second dimension move (the filled part of a cache).  What moves of a row must be contiguous, and
-    no two states may share memory."""
+    the states' second dimension move (the filled part of a cache).  What moves of a row must be contiguous and at
+    most 2^36 - 1024 bytes, and no two states may share memory."""
     _native.ops().reorder_states(states, parents, length)
