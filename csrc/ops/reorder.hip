@@ -4,7 +4,7 @@
 // some other beam wants, then writes the beams that change.  No other thread touches them, so no copy of the state
 // is needed, whatever the parents are.  A beam that stays is neither read for itself nor written.
 //
-// Bound by HBM.  1.43 GB of moves among 8 beams (caches of 3001 tokens) take 236 to 258 us on different cards, 5.5 to
+// Bound by HBM.  1.43 GB of moves among 8 beams (caches of 3001 tokens) take 236 to 252 us on different cards, 5.7 to
 // 6.1 TB/s.  How it got there, timed in one way on one card (277 us, 16 beams 289): the pieces go past the caches
 // (362 us without: nothing of a long state is read again before it is gone), and a workgroup is one wave with one
 // piece to a thread (four waves 310 us, four pieces 332).  Each piece read is stored to its children one by one:
